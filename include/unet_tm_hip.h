@@ -166,6 +166,53 @@ int mi_conv1x1_head_bwd(const void* x, int x_cstride, int x_coff, const float* w
                         int B, int H, int W, int Cin, int Cout, int relu_mask, int dtype, mi_stream s);
 size_t mi_conv1x1_head_ws_bytes(int Cin, int Cout);
 
+/* ------------------------------------------------------------------ dropout, group norm */
+/* Layers for blocks of a wider U-Net (the reference's blocks have neither).  Both take NHWC views like the layers
+ * above; channel strides and offsets are multiples of 16, pointers 16-byte aligned.  Padding channels of an input may
+ * hold anything, those of an output are written as zeros.  An empty batch (B = 0) is allowed.
+ *
+ * Dropout.  Whether a unit survives is a function of (seed, offset, unit number): nothing is stored, the backward
+ * pass is handed the same description again.  Unit number of element (b,y,x,c): ((b*H+y)*W+x)*mi_pad_channels(C)+c,
+ * or b*mi_pad_channels(C)+c with per_channel (whole feature maps), whatever the strides of the view, the dtype and the
+ * kernel.  Unit e has 16 bits, half e%2 of word (e/2)%4 of Philox4x32-10(counter = (e/8, offset), key = seed) and
+ * survives where they are below K = floor((1-p)*65536+0.5); survivors are multiplied by 65536/K, the others are zero
+ * (also where x is infinite or NaN).  p = 1 drops everything.
+ * offset_dev (may be NULL): device int64 added to offset when the kernel runs.  A captured graph replays with another
+ * mask once the caller has counted it up; it must not change between a forward and its backward pass. */
+typedef struct {
+  double p;                   /* probability of dropping, 0 .. 1, in steps of 2^-16 */
+  uint64_t seed, offset;
+  const int64_t* offset_dev;
+  int per_channel;
+} mi_dropout;
+/* y = residual + dropout(x); residual may be NULL; y may be x or the residual itself (the same view, not a shifted
+ * one).  The gradient with respect to x is the same call on dy without a residual, that of the residual is dy. */
+int mi_dropout_fwd(const void* x, int x_cstride, int x_coff, const void* residual, int r_cstride, int r_coff,
+                   void* y, int y_cstride, int y_coff, int B, int H, int W, int C, const mi_dropout* drop, int dtype, mi_stream s);
+
+/* Activation codes of the normalisation: identity, max(z,0), z*sigmoid(z), z*Phi(z) (the exact form, with erf). */
+#define MI_ACT_NONE 0
+#define MI_ACT_RELU 1
+#define MI_ACT_SILU 2
+#define MI_ACT_GELU 3
+/* y = dropout(act((x - mean) * rstd * gamma + beta)): torch's nn.GroupNorm(groups, C, eps), an activation and a
+ * dropout (drop may be NULL) in one operator.  gamma, beta: C floats each, or NULL (1 and 0).  mean, rstd
+ * (B*groups floats each) are written; the backward pass reads them.  C must be a multiple of groups.  y must not
+ * overlap x.  ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content. */
+int mi_group_norm_act_fwd(const void* x, int x_cstride, int x_coff, const float* gamma, const float* beta,
+                          void* y, int y_cstride, int y_coff, float* mean, float* rstd,
+                          int B, int H, int W, int C, int groups, int act, float eps, const mi_dropout* drop,
+                          void* ws, size_t ws_bytes, int dtype, mi_stream s);
+/* dx, and dgamma = alpha*sum + beta_acc*dgamma, dbeta likewise (either may be NULL).  x, mean, rstd, gamma, beta, act
+ * and drop as in the forward pass; ReLU has slope 0 at 0.  dx must not overlap x or dy.  Sums have a fixed order:
+ * the same call gives the same bits.  ws: mi_group_norm_ws_bytes(..., 1, ...) bytes, any content. */
+int mi_group_norm_act_bwd(const void* x, int x_cstride, int x_coff, const void* dy, int dy_cstride, int dy_coff,
+                          const float* gamma, const float* beta, const float* mean, const float* rstd,
+                          void* dx, int dx_cstride, int dx_coff, float* dgamma, float* dbeta, float alpha, float beta_acc,
+                          int B, int H, int W, int C, int groups, int act, const mi_dropout* drop,
+                          void* ws, size_t ws_bytes, int dtype, mi_stream s);
+size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backward, int dtype);
+
 /* ------------------------------------------------------------------ A6: MSE loss */
 /* nn.MSELoss() (train.py:498/:387) and the sums of test.py:39-43 in one pass.
  * out3 (device, 3 floats) = { mean((pred-y)^2), sum|pred-y|, sum (pred-y)^2 }.

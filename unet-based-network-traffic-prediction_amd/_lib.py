@@ -10,6 +10,7 @@ import os
 
 MI_F32, MI_BF16 = 0, 1
 MI_FWD_REPACK, MI_FWD_TRAIN = 1, 2
+MI_ACT_NONE, MI_ACT_RELU, MI_ACT_SILU, MI_ACT_GELU = 0, 1, 2, 3
 MI_OPT_GRAPH, MI_OPT_SERIAL_BACKWARD, MI_OPT_DEBUG_STREAMS, MI_OPT_PACK_ONE_STREAM, MI_OPT_NO_KSPLIT = 1, 2, 3, 4, 5
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -20,6 +21,11 @@ class UNetDesc(C.Structure):
     _fields_ = [("in_channels", C.c_int), ("out_channels", C.c_int), ("n_levels", C.c_int),
                 ("features", C.c_int * 8), ("batch", C.c_int), ("height", C.c_int), ("width", C.c_int),
                 ("out_h", C.c_int), ("out_w", C.c_int), ("dtype", C.c_int), ("need_input_grad", C.c_int)]
+
+
+class Dropout(C.Structure):
+    _fields_ = [("p", C.c_double), ("seed", C.c_uint64), ("offset", C.c_uint64), ("offset_dev", C.c_void_p),
+                ("per_channel", C.c_int)]
 
 
 _i, _f, _p, _sz, _i64 = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_int64
@@ -51,6 +57,10 @@ SIGNATURES = {
     "mi_conv1x1_head_fwd": (_i, _VIEW + [_p, _p, _p] + [_i] * 6 + [_p]),
     "mi_conv1x1_head_bwd": (_i, _VIEW + [_p, _p] + _VIEW + [_p, _p, _f, _f, _p, _sz] + [_i] * 7 + [_p]),
     "mi_conv1x1_head_ws_bytes": (_sz, [_i, _i]),
+    "mi_dropout_fwd": (_i, _VIEW + _VIEW + _VIEW + [_i] * 4 + [_p, _i, _p]),
+    "mi_group_norm_act_fwd": (_i, _VIEW + [_p, _p] + _VIEW + [_p, _p] + [_i] * 6 + [_f, _p, _p, _sz, _i, _p]),
+    "mi_group_norm_act_bwd": (_i, _VIEW + _VIEW + [_p] * 4 + _VIEW + [_p, _p, _f, _f] + [_i] * 6 + [_p, _p, _sz, _i, _p]),
+    "mi_group_norm_ws_bytes": (_sz, [_i] * 7),
     "mi_mse_fwd_bwd": (_i, [_p, _p, _i64, _p, _p, _f, _p, _p, _sz, _p]),
     "mi_mse_ws_bytes": (_sz, [_i64]),
     "mi_bilinear_fwd": (_i, [_p] + [_i64] * 4 + [_i, _p] + [_i64] * 4 + [_i] + [_i] * 6 + [_p]),

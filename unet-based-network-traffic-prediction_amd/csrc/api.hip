@@ -556,6 +556,71 @@ int mi_maxpool2_bwd(const void* x, int xcs, int xco, const void* dyp, int pcs, i
                              (hipStream_t)s);
 }
 
+// A view that the 16-byte kernels may touch: pad_ch(C) channels inside the stride, everything 16-byte aligned.
+static bool view_ok(const void* p, int cs, int co, int C) {
+  return p != nullptr && aligned16(p) && cs % 16 == 0 && co % 16 == 0 && co >= 0 && (int64_t)co + pad_ch(C) <= cs;
+}
+// Whether two views of one pixel count share an element (channel ranges of one buffer do not).
+static bool views_overlap(const void* p, int pcs, int pco, const void* q, int qcs, int qco, int64_t px, int C, int dtype) {
+  const int64_t es = elem_size(dtype), n = pad_ch(C) * es;
+  const int64_t p0 = (int64_t)(uintptr_t)p + pco * es, q0 = (int64_t)(uintptr_t)q + qco * es;
+  if (px <= 0 || p0 + (px - 1) * pcs * es + n <= q0 || q0 + (px - 1) * qcs * es + n <= p0) return false;
+  if (pcs != qcs) return true;
+  const int64_t pitch = pcs * es, d = ((p0 - q0) % pitch + pitch) % pitch;      // distance within a pixel
+  return d < n || pitch - d < n;
+}
+#define MI_NHWC_SHAPE(what)                                                                                              \
+  MI_REQUIRE(B >= 0 && H > 0 && W > 0 && C > 0 && C <= (1 << 24), what ": bad shape");                                   \
+  MI_REQUIRE((int64_t)H * W < (1ll << 31) && (int64_t)B * H * W < (1ll << 31), what ": pixel count out of range");       \
+  MI_REQUIRE(dtype == MI_F32 || dtype == MI_BF16, what ": bad dtype")
+int mi_dropout_fwd(const void* x, int xcs, int xco, const void* r, int rcs, int rco, void* y, int ycs, int yco, int B, int H,
+                   int W, int C, const mi_dropout* drop, int dtype, mi_stream s) {
+  MI_NHWC_SHAPE("dropout_fwd");
+  if (B == 0) return MI_OK;
+  MI_REQUIRE(view_ok(x, xcs, xco, C) && view_ok(y, ycs, yco, C) && (r == nullptr || view_ok(r, rcs, rco, C)),
+             "dropout_fwd: bad view (null, unaligned, or channels outside the stride)");
+  const int64_t px = (int64_t)B * H * W, es = elem_size(dtype);
+  auto same = [&](const void* p, int cs, int co) { return cs == ycs && (const char*)p + co * es == (const char*)y + yco * es; };
+  MI_REQUIRE(same(x, xcs, xco) || !views_overlap(x, xcs, xco, y, ycs, yco, px, C, dtype), "dropout_fwd: y overlaps x without being x");
+  MI_REQUIRE(r == nullptr || same(r, rcs, rco) || !views_overlap(r, rcs, rco, y, ycs, yco, px, C, dtype),
+             "dropout_fwd: y overlaps the residual without being it");
+  return launch_dropout(x, xcs, xco, r, rcs, rco, y, ycs, yco, B, H, W, C, drop, dtype, (hipStream_t)s);
+}
+size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backward, int dtype) {
+  if (B < 0 || H <= 0 || W <= 0 || C <= 0 || groups <= 0 || C % groups || (int64_t)H * W >= (1ll << 31)) return 0;
+  return group_norm_ws_bytes(B, H, W, C, groups, backward, dtype);
+}
+#define MI_NORM_ARGS(what)                                                                                               \
+  MI_NHWC_SHAPE(what);                                                                                                   \
+  MI_REQUIRE(groups > 0 && C % groups == 0, what ": the channel count must be a multiple of the group count");           \
+  MI_REQUIRE(act >= MI_ACT_NONE && act <= MI_ACT_GELU, what ": unknown activation");                                     \
+  MI_REQUIRE(B == 0 || (mean != nullptr && rstd != nullptr && ws != nullptr && ((uintptr_t)ws & 15) == 0),               \
+             what ": statistics or workspace missing or unaligned")
+int mi_group_norm_act_fwd(const void* x, int xcs, int xco, const float* gamma, const float* beta, void* y, int ycs, int yco,
+                          float* mean, float* rstd, int B, int H, int W, int C, int groups, int act, float eps,
+                          const mi_dropout* drop, void* ws, size_t ws_bytes, int dtype, mi_stream s) {
+  MI_NORM_ARGS("group_norm_act_fwd");
+  MI_REQUIRE(eps >= 0.f, "group_norm_act_fwd: eps must not be negative");
+  MI_REQUIRE(B == 0 || (view_ok(x, xcs, xco, C) && view_ok(y, ycs, yco, C)),
+             "group_norm_act_fwd: bad view (null, unaligned, or channels outside the stride)");
+  MI_REQUIRE(!views_overlap(x, xcs, xco, y, ycs, yco, (int64_t)B * H * W, C, dtype), "group_norm_act_fwd: y overlaps x");
+  return launch_group_norm_fwd(x, xcs, xco, gamma, beta, y, ycs, yco, mean, rstd, B, H, W, C, groups, act, eps, drop, ws,
+                               ws_bytes, dtype, (hipStream_t)s);
+}
+int mi_group_norm_act_bwd(const void* x, int xcs, int xco, const void* dy, int ycs, int yco, const float* gamma, const float* beta,
+                          const float* mean, const float* rstd, void* dx, int dcs, int dco, float* dgamma, float* dbeta,
+                          float alpha, float beta_acc, int B, int H, int W, int C, int groups, int act, const mi_dropout* drop,
+                          void* ws, size_t ws_bytes, int dtype, mi_stream s) {
+  MI_NORM_ARGS("group_norm_act_bwd");
+  MI_REQUIRE(B == 0 || (view_ok(x, xcs, xco, C) && view_ok(dy, ycs, yco, C) && view_ok(dx, dcs, dco, C)),
+             "group_norm_act_bwd: bad view (null, unaligned, or channels outside the stride)");
+  const int64_t px = (int64_t)B * H * W;
+  MI_REQUIRE(!views_overlap(x, xcs, xco, dx, dcs, dco, px, C, dtype) && !views_overlap(dy, ycs, yco, dx, dcs, dco, px, C, dtype),
+             "group_norm_act_bwd: dx overlaps x or dy");
+  return launch_group_norm_bwd(x, xcs, xco, dy, ycs, yco, gamma, beta, mean, rstd, dx, dcs, dco, dgamma, dbeta, alpha, beta_acc,
+                               B, H, W, C, groups, act, drop, ws, ws_bytes, dtype, (hipStream_t)s);
+}
+
 int mi_convt2x2_fwd(const void* x, int xcs, int xco, const void* wfwd, const float* bias, void* y, int ycs, int yco,
                     int B, int H, int W, int Cin, int Cout, int dtype, mi_stream s) {
   MI_REQUIRE(B > 0 && H > 0 && W > 0 && Cin > 0 && Cout > 0, "convt2x2_fwd: bad shape");

@@ -1,0 +1,101 @@
+// Dropout from a counter: what every kernel that drops shares.
+//
+// Whether a unit survives is a function of (seed, offset, unit number) alone, so the mask is never stored: the
+// backward pass, a fused kernel and a stand-alone one work it out again.  The generator is Philox4x32-10 (Salmon,
+// Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC11): ten rounds of two 32 x 32 -> 64
+// multiplies over a 128-bit counter.  Unit e takes 16 of the 128 bits of call e / 8: half e & 1 of word (e >> 1) & 3.
+// One call then serves the eight bf16 values of a 16-byte vector, and its ~150 instructions hide behind the vector's
+// 32 bytes of traffic (copy of 537 MB with a call per vector: 5.85 TB/s, without: 5.81); with 32 bits a unit they
+// would not.  The price: p counts in steps of 2^-16.  The scale follows the rounded p, so the expectation is exact.
+#pragma once
+#include "common.h"
+
+namespace mi {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+struct DropArgs {
+  int on;                      // 0: nothing is dropped
+  int per_channel;             // one unit per (image, channel) instead of one per element
+  uint32_t keep;               // a unit survives where its 16 bits are below this (0 .. 65536)
+  float scale;                 // 65536 / keep
+  uint32_t k0, k1;             // seed
+  uint64_t offset;
+  const int64_t* offset_dev;   // optional, added to offset (read on the device)
+};
+// Checks and converts the caller's description; null = no dropout.
+int make_drop_args(const mi_dropout* d, DropArgs* out);
+
+__device__ __forceinline__ uint64_t drop_offset(const DropArgs& d) {
+  return d.offset + (d.offset_dev != nullptr ? (uint64_t)*d.offset_dev : 0);
+}
+// Four words of call number n.
+__device__ __forceinline__ u32x4_t drop_words(uint64_t n, uint64_t offset, uint32_t k0, uint32_t k1) {
+  uint32_t a = (uint32_t)n, b = (uint32_t)(n >> 32), c = (uint32_t)offset, d = (uint32_t)(offset >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p = (uint64_t)a * 0xD2511F53u, q = (uint64_t)c * 0xCD9E8D57u;
+    a = (uint32_t)(q >> 32) ^ b ^ k0;
+    b = (uint32_t)q;
+    c = (uint32_t)(p >> 32) ^ d ^ k1;
+    d = (uint32_t)p;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return u32x4_t{a, b, c, d};
+}
+// Keep bits (bit j = unit j survives) of the N units from unit e on, e a multiple of N, N = 4 or 8.
+template <int N>
+__device__ __forceinline__ uint32_t drop_bits(const DropArgs& d, uint64_t offset, uint64_t e) {
+  const u32x4_t w = drop_words(e >> 3, offset, d.k0, d.k1);
+  uint32_t bits = 0;
+  if constexpr (N == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      bits |= ((w[j] & 0xffffu) < d.keep ? 1u : 0u) << (2 * j) | ((w[j] >> 16) < d.keep ? 1u : 0u) << (2 * j + 1);
+  } else {
+    const uint32_t w0 = e & 4 ? w[2] : w[0], w1 = e & 4 ? w[3] : w[1];
+    bits = ((w0 & 0xffffu) < d.keep ? 1u : 0u) | ((w0 >> 16) < d.keep ? 2u : 0u) | ((w1 & 0xffffu) < d.keep ? 4u : 0u) |
+           ((w1 >> 16) < d.keep ? 8u : 0u);
+  }
+  return bits;
+}
+
+// ---------------------------------------------------------------- 16-byte vectors of activations
+template <typename T> struct ActVec;
+template <> struct ActVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(u32x4_t v, float* f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(v[j]);
+  }
+  static __device__ __forceinline__ u32x4_t pack(const float* f) {
+    return u32x4_t{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+  }
+};
+template <> struct ActVec<__bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(u32x4_t v, float* f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[2 * j] = __uint_as_float(v[j] << 16);
+      f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ u32x4_t pack(const float* f) {   // round to nearest even: one rounding, of the stored result
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    u32x4_t v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)f[2 * j], (__bf16)f[2 * j + 1]});
+    return v;
+  }
+};
+// Streamed: nothing in these kernels comes back to a line it has read or written.
+template <typename T> __device__ __forceinline__ u32x4_t load_stream(const T* p) {
+  return __builtin_nontemporal_load((const u32x4_t*)p);
+}
+template <typename T> __device__ __forceinline__ void store_stream(T* p, u32x4_t v) {
+  __builtin_nontemporal_store(v, (u32x4_t*)p);
+}
+
+}  // namespace mi

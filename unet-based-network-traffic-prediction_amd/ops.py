@@ -7,11 +7,14 @@ current torch stream and returns torch tensors it allocated; nothing here comput
 with torch ops."""
 from __future__ import annotations
 
+import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
 
-from ._lib import MI_BF16, MI_F32, check, lib
+from ._lib import MI_ACT_GELU, MI_ACT_NONE, MI_ACT_RELU, MI_ACT_SILU, MI_BF16, MI_F32, check, lib
+from ._lib import Dropout as _DropoutDesc
 
 
 def pad_ch(c: int) -> int:
@@ -205,6 +208,172 @@ def head_bwd(x, weight, dpred, Cin, Cout, relu_mask=True, alpha=1.0, beta=0.0):
                                     dW.data_ptr(), db.data_ptr(), alpha, beta, ws.data_ptr(), nbytes, B, H, W, Cin, Cout,
                                     int(relu_mask), mi_dtype(x.dtype), _stream()), "head_bwd")
     return dx, dW, db
+
+
+# ------------------------------------------------------------------ dropout, group norm
+ACTIVATIONS = {"none": MI_ACT_NONE, "relu": MI_ACT_RELU, "silu": MI_ACT_SILU, "gelu": MI_ACT_GELU}
+
+
+class Drop:
+    """What is dropped: a function of these values and of an element's place alone, so no mask is stored and the
+    backward pass takes the same object.
+
+    ``p`` counts in steps of 2^-16 (survivors are scaled by the rounded value).  ``seed`` and ``offset`` are integers
+    in [0, 2^64); layers of one step take different offsets (or seeds).  ``offset_dev`` (a one-element int64 tensor on
+    the GPU) is added to ``offset`` when a kernel runs: a captured graph replays with new masks if it is counted up
+    between replays.  ``per_channel`` drops whole feature maps."""
+
+    __slots__ = ("p", "seed", "offset", "offset_dev", "per_channel", "_desc")
+
+    def __init__(self, p: float, seed: int, offset: int = 0, offset_dev: Optional[torch.Tensor] = None,
+                 per_channel: bool = False):
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout: p must be between 0 and 1, got {p}")
+        if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+            raise ValueError("dropout: seed and offset must be in [0, 2^64)")
+        if offset_dev is not None and (offset_dev.dtype != torch.int64 or offset_dev.numel() != 1 or not offset_dev.is_cuda):
+            raise ValueError("dropout: offset_dev must be a one-element int64 tensor on the GPU")
+        self.p, self.seed, self.offset, self.offset_dev, self.per_channel = p, seed, offset, offset_dev, per_channel
+        self._desc = _DropoutDesc(p, seed, offset, offset_dev.data_ptr() if offset_dev is not None else None, int(per_channel))
+
+
+def _drop_ref(drop: Optional[Drop], dev: torch.device):
+    if drop is None:
+        return None
+    if drop.offset_dev is not None and drop.offset_dev.device != dev:
+        raise RuntimeError(f"dropout: offset_dev is on {drop.offset_dev.device}, the activation on {dev}")
+    return ctypes.byref(drop._desc)
+
+
+def _nhwc(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> None:
+    """Refuses what is no dense (B, H, W, channels) activation, or not of the size, type and device of ``like``."""
+    if not t.is_cuda:
+        _need_cuda(t)
+    if t.dim() != 4 or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous (B, H, W, channels) tensor, got shape {tuple(t.shape)}, strides {t.stride()}")
+    if like is not None and (t.shape[:3] != like.shape[:3] or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{what}: {tuple(t.shape[:3])} {t.dtype} on {t.device} does not go with "
+                         f"{tuple(like.shape[:3])} {like.dtype} on {like.device}")
+
+
+def _channel_vector(t: Optional[torch.Tensor], n: int, dev: torch.device, what: str):
+    """Pointer of an fp32 tensor of n values on ``dev`` (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: expected {n} contiguous float32 values on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+class _NoGuard:
+    __slots__ = ()
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _on(dev: torch.device):
+    """Context in which kernels are launched on ``dev``; free when it is the current device already."""
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _activation(act: str) -> int:
+    try:
+        return ACTIVATIONS[act]
+    except KeyError:
+        raise ValueError(f"unknown activation {act!r} ({', '.join(ACTIVATIONS)})") from None
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_ws_bytes(B, H, W, Cc, groups, backward, dt) -> int:
+    return lib().mi_group_norm_ws_bytes(B, H, W, Cc, groups, backward, dt)
+
+
+def dropout_fwd(x, C, drop: Optional[Drop], residual=None, x_coff=0, residual_coff=0, out=None, out_coff=0):
+    """``residual + dropout(x)`` (NHWC, C of the channels from ``x_coff`` on); ``out`` may be x or the residual;
+    without a ``drop`` nothing is dropped."""
+    _nhwc(x, "dropout")
+    B, H, W, cs = x.shape
+    dev = x.device
+    rv = (None, 0, 0)
+    if residual is not None:
+        _nhwc(residual, "dropout residual", x)
+        rv = (residual.data_ptr(), residual.shape[3], residual_coff)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((B, H, W, pad_ch(C)), device=dev, dtype=x.dtype)
+        else:
+            _nhwc(out, "dropout out", x)
+        check(lib().mi_dropout_fwd(x.data_ptr(), cs, x_coff, *rv, out.data_ptr(), out.shape[3], out_coff, B, H, W, C,
+                                   _drop_ref(drop, dev), mi_dtype(x.dtype), torch.cuda.current_stream(dev).cuda_stream),
+              "dropout_fwd")
+    return out
+
+
+def dropout_bwd(dy, C, drop: Drop, dy_coff=0, out=None, out_coff=0):
+    """Gradient with respect to x (that of the residual is dy itself)."""
+    return dropout_fwd(dy, C, drop, x_coff=dy_coff, out=out, out_coff=out_coff)
+
+
+def group_norm_act_fwd(x, C, groups, weight=None, bias=None, act="none", eps=1e-5, drop: Optional[Drop] = None, x_coff=0,
+                       out=None, out_coff=0):
+    """``dropout(act(group_norm(x)))`` of the C channels from ``x_coff`` on.  Returns (y, mean, rstd): the statistics
+    (B, groups) are what the backward pass needs besides x."""
+    _nhwc(x, "group_norm_act")
+    B, H, W, cs = x.shape
+    dev, dt = x.device, mi_dtype(x.dtype)
+    code = _activation(act)
+    wp, bp = _channel_vector(weight, C, dev, "group_norm_act weight"), _channel_vector(bias, C, dev, "group_norm_act bias")
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError(f"group_norm_act: {C} channels do not split into {groups} groups")
+    with _on(dev):
+        if out is None:
+            out = torch.empty((B, H, W, pad_ch(C)), device=dev, dtype=x.dtype)
+        else:
+            _nhwc(out, "group_norm_act out", x)
+        stats = torch.empty((2, B, groups), device=dev, dtype=torch.float32)
+        nbytes = _norm_ws_bytes(B, H, W, C, groups, 0, dt)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        sp = stats.data_ptr()
+        check(lib().mi_group_norm_act_fwd(x.data_ptr(), cs, x_coff, wp, bp, out.data_ptr(), out.shape[3], out_coff, sp,
+                                          sp + 4 * B * groups, B, H, W, C, groups, code, eps, _drop_ref(drop, dev), ws.data_ptr(),
+                                          nbytes, dt, torch.cuda.current_stream(dev).cuda_stream), "group_norm_act_fwd")
+    return out, stats[0], stats[1]
+
+
+def group_norm_act_bwd(x, dy, mean, rstd, C, groups, weight=None, bias=None, act="none", drop: Optional[Drop] = None, x_coff=0,
+                       dy_coff=0, dweight=None, dbias=None, alpha=1.0, beta=0.0):
+    """(dx, dweight, dbias) from what the forward pass was given and returned.  ``dweight`` / ``dbias`` are None where
+    the parameter is; tensors passed in receive ``alpha * gradient + beta * themselves``."""
+    _nhwc(x, "group_norm_act")
+    _nhwc(dy, "group_norm_act dy", x)
+    B, H, W, cs = x.shape
+    dev, dt = x.device, mi_dtype(x.dtype)
+    code = _activation(act)
+    wp, bp = _channel_vector(weight, C, dev, "group_norm_act weight"), _channel_vector(bias, C, dev, "group_norm_act bias")
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError(f"group_norm_act: {C} channels do not split into {groups} groups")
+    mp, rp = (_channel_vector(t, B * groups, dev, "group_norm_act statistics") for t in (mean, rstd))
+    with _on(dev):
+        dx = torch.empty((B, H, W, pad_ch(C)), device=dev, dtype=x.dtype)
+        if weight is not None and dweight is None:
+            dweight = torch.empty_like(weight) if beta == 0.0 else torch.zeros_like(weight)
+        if bias is not None and dbias is None:
+            dbias = torch.empty_like(bias) if beta == 0.0 else torch.zeros_like(bias)
+        gp, hp = _channel_vector(dweight, C, dev, "group_norm_act dweight"), _channel_vector(dbias, C, dev, "group_norm_act dbias")
+        nbytes = _norm_ws_bytes(B, H, W, C, groups, 1, dt)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        check(lib().mi_group_norm_act_bwd(x.data_ptr(), cs, x_coff, dy.data_ptr(), dy.shape[3], dy_coff, wp, bp, mp, rp,
+                                          dx.data_ptr(), dx.shape[3], 0, gp, hp, alpha, beta, B, H, W, C, groups, code,
+                                          _drop_ref(drop, dev), ws.data_ptr(), nbytes, dt,
+                                          torch.cuda.current_stream(dev).cuda_stream), "group_norm_act_bwd")
+    return dx, dweight, dbias
 
 
 # ------------------------------------------------------------------ loss
