@@ -4,9 +4,9 @@
 // backward pass, a fused kernel and a stand-alone one work it out again.  The generator is Philox4x32-10 (Salmon,
 // Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC11): ten rounds of two 32 x 32 -> 64
 // multiplies over a 128-bit counter.  Unit e takes 16 of the 128 bits of call e / 8: half e & 1 of word (e >> 1) & 3.
-// One call then serves the eight bf16 values of a 16-byte vector, and its ~150 instructions hide behind the vector's
-// 32 bytes of traffic (copy of 537 MB with a call per vector: 5.85 TB/s, without: 5.81); with 32 bits a unit they
-// would not.  The price: p counts in steps of 2^-16.  The scale follows the rounded p, so the expectation is exact.
+// One call then serves the eight bf16 values of a 16-byte vector: 20 multiplies (4 cycles a wave each) and 20 three-way
+// xors (2 cycles), a fifth of the time that the vector's 32 bytes of traffic take (537 MB copied with a call per
+// vector: 5.85 TB/s, without: 5.81); with 32 bits a unit it would be two fifths, on top of a norm's own work.  The price: p counts in steps of 2^-16.  The scale follows the rounded p, so the expectation is exact.
 #pragma once
 #include "common.h"
 
@@ -29,37 +29,54 @@ int make_drop_args(const mi_dropout* d, DropArgs* out);
 __device__ __forceinline__ uint64_t drop_offset(const DropArgs& d) {
   return d.offset + (d.offset_dev != nullptr ? (uint64_t)*d.offset_dev : 0);
 }
-// Four words of call number n.
+// Four words of call number n, the halves as signed numbers (each has its top bit turned: u < keep then is a signed
+// comparison; for two of the words the turn rides in the last round's key).
 __device__ __forceinline__ u32x4_t drop_words(uint64_t n, uint64_t offset, uint32_t k0, uint32_t k1) {
   uint32_t a = (uint32_t)n, b = (uint32_t)(n >> 32), c = (uint32_t)offset, d = (uint32_t)(offset >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p = (uint64_t)a * 0xD2511F53u, q = (uint64_t)c * 0xCD9E8D57u;
-    a = (uint32_t)(q >> 32) ^ b ^ k0;
+    const uint32_t turn = r == 9 ? 0x80008000u : 0u;
+    a = __builtin_amdgcn_bitop3_b32((uint32_t)(q >> 32), b, k0 ^ turn, 0x96);    // three-way xor
     b = (uint32_t)q;
-    c = (uint32_t)(p >> 32) ^ d ^ k1;
+    c = __builtin_amdgcn_bitop3_b32((uint32_t)(p >> 32), d, k1 ^ turn, 0x96);
     d = (uint32_t)p;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return u32x4_t{a, b, c, d};
+  return u32x4_t{a, b ^ 0x80008000u, c, d ^ 0x80008000u};
 }
-// Keep bits (bit j = unit j survives) of the N units from unit e on, e a multiple of N, N = 4 or 8.
-template <int N>
-__device__ __forceinline__ uint32_t drop_bits(const DropArgs& d, uint64_t offset, uint64_t e) {
-  const u32x4_t w = drop_words(e >> 3, offset, d.k0, d.k1);
-  uint32_t bits = 0;
-  if constexpr (N == 8) {
+// The keep bits of I vectors of N units, collected two at a time: the saturated difference of a half and `keep` has the
+// answer in its sign.  The bits of a thread's vectors are worked out while their loads are in flight and cost a
+// register per 32 units until they are used.
+template <int I, int N>
+struct KeepBits {
+  static constexpr int kWords = I * N / 2, kRegs = (kWords + 15) / 16;
+  uint32_t r[kRegs];
+  // vector i (a literal after unrolling, 0, 1, 2, ...): its units start at e, a multiple of N
+  __device__ __forceinline__ void add(int i, const DropArgs& d, uint64_t offset, uint64_t e) {
+    const u32x4_t w = drop_words(e >> 3, offset, d.k0, d.k1);
+    typedef short s16x2_t __attribute__((ext_vector_type(2)));
+    const s16x2_t k = __builtin_bit_cast(s16x2_t, (d.keep ^ 0x8000u) * 0x10001u);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      bits |= ((w[j] & 0xffffu) < d.keep ? 1u : 0u) << (2 * j) | ((w[j] >> 16) < d.keep ? 1u : 0u) << (2 * j + 1);
-  } else {
-    const uint32_t w0 = e & 4 ? w[2] : w[0], w1 = e & 4 ? w[3] : w[1];
-    bits = ((w0 & 0xffffu) < d.keep ? 1u : 0u) | ((w0 >> 16) < d.keep ? 2u : 0u) | ((w1 & 0xffffu) < d.keep ? 4u : 0u) |
-           ((w1 >> 16) < d.keep ? 8u : 0u);
+    for (int h = 0; h < N / 2; ++h) {
+      const uint32_t word = N == 8 ? w[h] : (e & 4 ? w[2 + h] : w[h]);
+      const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(s16x2_t, word), k));
+      const int at = i * (N / 2) + h;
+      r[at / 16] = at % 16 == 0 ? t & 0x80008000u : r[at / 16] >> 1 | (t & 0x80008000u);
+    }
   }
-  return bits;
-}
+  // f where unit j of vector i survives, +0 where it does not
+  __device__ __forceinline__ float kept(int i, int j, float f) const {
+    const int at = i * (N / 2) + j / 2, in_reg = at / 16 < kRegs - 1 ? 16 : kWords - 16 * (kRegs - 1);
+    const int bit = (j & 1) * 16 + 16 - in_reg + at % 16;
+    return __uint_as_float(__float_as_uint(f) & (uint32_t)((int32_t)(r[at / 16] << (31 - bit)) >> 31));
+  }
+  __device__ __forceinline__ void keep_all() {
+#pragma unroll
+    for (int k = 0; k < kRegs; ++k) r[k] = ~0u;
+  }
+};
 
 // ---------------------------------------------------------------- 16-byte vectors of activations
 template <typename T> struct ActVec;

@@ -57,18 +57,23 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropoutArgs a) {
     vx[u] = load_stream(x + px[u] * a.xcs + a.xco + c[u]);
     if (RES) vr[u] = load_stream(r + px[u] * a.rcs + a.rco + c[u]);
   }
-  const uint64_t offset = drop_offset(a.drop);
+  KeepBits<kU, N> keep;
+  if (a.drop.on) {
+    const uint64_t offset = drop_offset(a.drop);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint64_t row = a.drop.per_channel ? fdiv((uint32_t)px[u], a.d_px) : (uint64_t)px[u];
+      keep.add(u, a.drop, offset, row * (uint32_t)(a.nv * N) + c[u]);
+    }
+  } else {
+    keep.keep_all();
+  }
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
     float f[N], g[N];
     ActVec<T>::unpack(vx[u], f);
-    uint32_t bits = 0xff;
-    if (a.drop.on) {
-      const uint64_t row = a.drop.per_channel ? fdiv((uint32_t)px[u], a.d_px) : (uint64_t)px[u];
-      bits = drop_bits<N>(a.drop, offset, row * (uint32_t)(a.nv * N) + c[u]);
-    }
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = bits >> j & 1 ? f[j] * a.drop.scale : 0.f;   // a dropped NaN is a zero
+    for (int j = 0; j < N; ++j) f[j] = keep.kept(u, j, f[j] * a.drop.scale);       // a dropped NaN is a zero
     if (RES) {
       ActVec<T>::unpack(vr[u], g);
 #pragma unroll
