@@ -64,6 +64,8 @@ struct KeepBits {
       const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(s16x2_t, word), k));
       const int at = i * (N / 2) + h;
       r[at / 16] = at % 16 == 0 ? t & 0x80008000u : r[at / 16] >> 1 | (t & 0x80008000u);
+      // the compiler would rather keep every t than read its sign back from here
+      if (at % 16 == 15 || at == kWords - 1) asm("" : "+v"(r[at / 16]));
     }
   }
   // f where unit j of vector i survives, +0 where it does not
@@ -72,6 +74,11 @@ struct KeepBits {
     const int bit = (j & 1) * 16 + 16 - in_reg + at % 16;
     return __uint_as_float(__float_as_uint(f) & (uint32_t)((int32_t)(r[at / 16] << (31 - bit)) >> 31));
   }
+  // no bit is looked at before this point
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (int k = 0; k < kRegs; ++k) asm volatile("" : "+v"(r[k]));
+  }
   __device__ __forceinline__ void keep_all() {
 #pragma unroll
     for (int k = 0; k < kRegs; ++k) r[k] = ~0u;
@@ -79,31 +86,53 @@ struct KeepBits {
 };
 
 // ---------------------------------------------------------------- 16-byte vectors of activations
+// N values; in groups of 4 (group h of a bf16 vector: words 2h and 2h + 1), so that a kernel which has little room for
+// unpacked values can take one group after the other.
 template <typename T> struct ActVec;
 template <> struct ActVec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(u32x4_t v, float* f) {
+  static __device__ __forceinline__ void unpack4(u32x4_t v, int, float* f) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(v[j]);
   }
+  static __device__ __forceinline__ void pack4(const float* f, int, u32x4_t& v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(f[j]);
+  }
+  static __device__ __forceinline__ void pack4_exact(const float* f, int, u32x4_t& v) { pack4(f, 0, v); }
+  static __device__ __forceinline__ void unpack(u32x4_t v, float* f) { unpack4(v, 0, f); }
   static __device__ __forceinline__ u32x4_t pack(const float* f) {
-    return u32x4_t{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    u32x4_t v;
+    pack4(f, 0, v);
+    return v;
   }
 };
 template <> struct ActVec<__bf16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(u32x4_t v, float* f) {
+  static __device__ __forceinline__ void unpack4(u32x4_t v, int h, float* f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[2 * j] = __uint_as_float(v[j] << 16);
-      f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
+    for (int j = 0; j < 2; ++j) {
+      f[2 * j] = __uint_as_float(v[2 * h + j] << 16);
+      f[2 * j + 1] = __uint_as_float(v[2 * h + j] & 0xffff0000u);
     }
   }
-  static __device__ __forceinline__ u32x4_t pack(const float* f) {   // round to nearest even: one rounding, of the stored result
+  static __device__ __forceinline__ void pack4(const float* f, int h, u32x4_t& v) {   // to nearest even: one rounding, of the stored result
     typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-    u32x4_t v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)f[2 * j], (__bf16)f[2 * j + 1]});
+    for (int j = 0; j < 2; ++j) v[2 * h + j] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)f[2 * j], (__bf16)f[2 * j + 1]});
+  }
+  static __device__ __forceinline__ void pack4_exact(const float* f, int h, u32x4_t& v) {   // of values that are bf16 already
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[2 * h + j] = __builtin_amdgcn_perm(__float_as_uint(f[2 * j + 1]), __float_as_uint(f[2 * j]), 0x07060302);
+  }
+  static __device__ __forceinline__ void unpack(u32x4_t v, float* f) {
+    unpack4(v, 0, f);
+    unpack4(v, 1, f + 4);
+  }
+  static __device__ __forceinline__ u32x4_t pack(const float* f) {
+    u32x4_t v;
+    pack4(f, 0, v);
+    pack4(f + 4, 1, v);
     return v;
   }
 };

@@ -4,10 +4,10 @@
 
 namespace mi {
 
-int launch_gn_fwd_f32(const NormArgs& a, hipStream_t s);
-int launch_gn_fwd_bf16(const NormArgs& a, hipStream_t s);
-int launch_gn_bwd_f32(const NormArgs& a, hipStream_t s);
-int launch_gn_bwd_bf16(const NormArgs& a, hipStream_t s);
+int launch_gn_fwd_f32(const NormArgs& a, const Slab* sl, hipStream_t s);
+int launch_gn_fwd_bf16(const NormArgs& a, const Slab* sl, hipStream_t s);
+int launch_gn_bwd_f32(const NormArgs& a, const Slab* sl, hipStream_t s);
+int launch_gn_bwd_bf16(const NormArgs& a, const Slab* sl, hipStream_t s);
 
 // One wave joins the tiles and pieces of a group.  Piece k of an image's tile covers channels k*q .. k*q + q - 1.
 __global__ __launch_bounds__(64) void gn_join_kernel(const NormArgs a) {
@@ -61,29 +61,35 @@ __global__ __launch_bounds__(64) void gn_bwd_join_kernel(const NormArgs a, int p
   const float n = (float)g.P * (float)g.cg;
   if (threadIdx.x == 0) a.moments[blockIdx.x] = make_float2(m1 / n, m2 / n);
 }
-// Sums over the images in a fixed order: a workgroup takes 8 channels, 32 threads share a channel's images.
-__global__ __launch_bounds__(256) void gn_param_grads_kernel(const NormArgs a) {
-  __shared__ float2 shared[256];
+// Sums the rows of channel sums in a fixed order: a workgroup takes 8 channels (one 64-byte piece of a row), 128 threads
+// share a channel's rows.
+__global__ __launch_bounds__(1024) void gn_param_grads_kernel(const NormArgs a) {
+  __shared__ float2 shared[16][8];
   const int k = threadIdx.x & 7, r = threadIdx.x >> 3, c = blockIdx.x * 8 + k;
   float2 s = make_float2(0.f, 0.f);
-  if (c < a.g.C)
-    for (int b = r; b < a.g.B; b += 32) {
-      const float2 p = a.chan[(int64_t)b * a.g.C + c];
+  if (c < a.g.C) {
+    for (int row = r; row < a.chan_rows; row += 128) {
+      const float2 p = a.chan[(int64_t)row * a.chan_stride + c];
       s.x += p.x;
       s.y += p.y;
     }
-  shared[threadIdx.x] = s;
+  }
+#pragma unroll
+  for (int o = 32; o >= 8; o >>= 1) {
+    s.x += __shfl_xor(s.x, o, 64);
+    s.y += __shfl_xor(s.y, o, 64);
+  }
+  if ((threadIdx.x & 63) < 8) shared[threadIdx.x >> 6][k] = s;
   __syncthreads();
-  if (r == 0 && c < a.g.C) {
-    for (int i = 1; i < 32; ++i) {
-      s.x += shared[i * 8 + k].x;
-      s.y += shared[i * 8 + k].y;
+  if (threadIdx.x < 8 && c < a.g.C) {
+    for (int w = 1; w < 16; ++w) {
+      s.x += shared[w][k].x;
+      s.y += shared[w][k].y;
     }
     if (a.dgamma) a.dgamma[c] = a.ga * s.y + (a.gb != 0.f ? a.gb * a.dgamma[c] : 0.f);
     if (a.dbeta) a.dbeta[c] = a.ga * s.x + (a.gb != 0.f ? a.gb * a.dbeta[c] : 0.f);
   }
 }
-
 // Fills the words that parts exchange (a kernel, not a memset: the call may be captured into a graph).
 __global__ __launch_bounds__(256) void gn_empty_kernel(uint64_t* words, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) words[i] = kEmpty;
@@ -97,7 +103,7 @@ void launch_gn_bwd_join(const NormArgs& a, int padded, hipStream_t s) {
   hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.g.B * a.g.G), dim3(64), 0, s, a, padded);
 }
 void launch_gn_param_grads(const NormArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(gn_param_grads_kernel, dim3((a.g.C + 7) / 8), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(gn_param_grads_kernel, dim3((a.g.C + 7) / 8), dim3(1024), 0, s, a);
 }
 
 // ---------------------------------------------------------------- host
@@ -127,13 +133,11 @@ static int pow2_ceil(int64_t v) {
   while (p < v) p <<= 1;
   return p;
 }
-// How the slab kernel divides the work, or false where it does not apply.
-constexpr int64_t kPartVectors = 512 * 8;    // 64 KB in a workgroup's registers
+// How the slab kernels divide the work, or false where they do not apply.
 constexpr int kMaxParts = 64;                // lanes of the wave that joins them
 constexpr int kPolls = 4096;
-bool choose_slab(const NormGeom& g, int N, Slab* out) {
-  int unit = g.cg / gcd_int(g.cg, N);                            // vectors after which a group ends with a vector
-  if (unit > g.nv) unit = g.nv;
+static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
+  const int unit = g.cg / gcd_int(g.cg, N) < g.nv ? g.cg / gcd_int(g.cg, N) : g.nv;   // vectors after which a group ends with a vector
   if (unit > 64) return false;
   Slab s{};
   int64_t cv = g.nv <= 64 ? g.nv : unit * (64 / unit);
@@ -148,22 +152,21 @@ bool choose_slab(const NormGeom& g, int N, Slab* out) {
   while ((1 << s.log_lanes) < s.lanes) ++s.log_lanes;
   s.chunks = (int)((g.nv + cv - 1) / cv);
   const int64_t vectors = (int64_t)g.P * s.lanes;
-  const int64_t parts = (vectors + kPartVectors - 1) / kPartVectors;
-  if (parts > kMaxParts) return false;
-  if (parts == 1) {
-    s.iters = vectors <= s.lanes ? 1 : (vectors <= 2048 ? 4 : 8);
-    s.tpi = pow2_ceil((vectors + s.iters - 1) / s.iters);
-    if (s.tpi < s.lanes) s.tpi = s.lanes;
-  } else {
-    s.iters = 8;
-    s.tpi = 512;
-  }
+  // as many vectors a thread as its registers hold where that leaves every CU a workgroup, else 4: less time for each
+  const int most = backward ? 8 : 16;
+  s.iters = vectors <= s.lanes ? 1 : ((int64_t)g.B * s.chunks * vectors < 256 * most * kSlabThreads ? 4 : most);
+  s.tpi = vectors < (int64_t)s.iters * kSlabThreads ? pow2_ceil((vectors + s.iters - 1) / s.iters) : kSlabThreads;
+  if (s.tpi < s.lanes) s.tpi = s.lanes;
   while ((1 << s.log_tpi) < s.tpi) ++s.log_tpi;
   s.rows = s.tpi / s.lanes;
-  s.parts = (g.P + s.rows * s.iters - 1) / (s.rows * s.iters);
+  const int64_t parts = (g.P + (int64_t)s.rows * s.iters - 1) / ((int64_t)s.rows * s.iters);
+  if (parts > kMaxParts) return false;
+  s.parts = (int)parts;
   while ((1 << s.log_parts) < s.parts) ++s.log_parts;
   s.nb = 1;
-  if (s.parts == 1) while (s.nb * s.tpi < 256 && s.nb < g.B) s.nb *= 2;
+  if (s.parts == 1) {
+    while (s.nb * s.tpi < kSlabThreads && s.nb < g.B) s.nb *= 2;
+  }
   s.img_blocks = (g.B + s.nb - 1) / s.nb;
   s.threads = s.nb * s.tpi < 64 ? 64 : s.nb * s.tpi;
   const int ppg = g.cg / g.q;
@@ -176,17 +179,20 @@ bool choose_slab(const NormGeom& g, int N, Slab* out) {
   *out = s;
   return true;
 }
+static size_t slab_rows(const Slab& s) { return (size_t)s.img_blocks * s.parts; }   // rows of channel sums
 static size_t fwd_part_bytes(const NormGeom& g) { return (size_t)g.B * g.tiles * g.nv * g.n_slots * sizeof(float4); }
 static size_t bwd_part_bytes(const NormGeom& g, int dtype) {
   return (size_t)g.B * g.tiles * g.nv * (dtype == MI_BF16 ? 8 : 4) * sizeof(float2);
 }
 size_t group_norm_ws_bytes(int B, int H, int W, int C, int G, int backward, int dtype) {
   const NormGeom g = norm_geom(B, H, W, C, G, dtype);
+  const int N = dtype == MI_BF16 ? 8 : 4;
+  Slab s;
   if (!backward) {
-    Slab s;
-    if (choose_slab(g, dtype == MI_BF16 ? 8 : 4, &s)) return s.parts > 1 ? slab_words(g, s) * sizeof(uint64_t) : 16;
+    if (choose_slab(g, N, false, &s)) return s.parts > 1 ? slab_words(g, s) * sizeof(uint64_t) : 16;
     return fwd_part_bytes(g) + 16;
   }
+  if (choose_slab(g, N, true, &s)) return (s.parts > 1 ? slab_words(g, s) / 2 * sizeof(uint64_t) : 0) + slab_rows(s) * C * sizeof(float2) + 16;
   return bwd_part_bytes(g, dtype) + ((size_t)B * C + (size_t)B * G) * sizeof(float2) + 16;
 }
 
@@ -204,6 +210,8 @@ int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, c
   a.g = norm_geom(B, H, W, C, G, dtype);
   if ((rc = check_range(a.g, "group_norm_act_fwd"))) return rc;
   if (B == 0) return MI_OK;
+  Slab slab;
+  const Slab* sl = choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, false, &slab) ? &slab : nullptr;
   if (ws_bytes < group_norm_ws_bytes(B, H, W, C, G, 0, dtype)) return fail(MI_ESIZE, "group_norm_act_fwd: workspace too small");
   a.x = x; a.xcs = xcs; a.xco = xco;
   a.out = y; a.ocs = ycs; a.oco = yco;
@@ -211,7 +219,7 @@ int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, c
   a.act = act; a.eps = eps;
   a.part = (float2*)ws;
   a.words = (uint64_t*)ws;
-  return dtype == MI_BF16 ? launch_gn_fwd_bf16(a, s) : launch_gn_fwd_f32(a, s);
+  return dtype == MI_BF16 ? launch_gn_fwd_bf16(a, sl, s) : launch_gn_fwd_f32(a, sl, s);
 }
 int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int ycs, int yco, const float* gamma, const float* beta,
                           const float* mean, const float* rstd, void* dx, int dcs, int dco, float* dgamma, float* dbeta,
@@ -228,11 +236,22 @@ int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int y
   a.out = dx; a.ocs = dcs; a.oco = dco;
   a.gamma = gamma; a.beta = beta; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.act = act;
-  a.part = (float2*)ws;
-  a.chan = a.part + bwd_part_bytes(a.g, dtype) / sizeof(float2);
-  a.moments = a.chan + (size_t)B * C;
+  Slab slab;
+  const Slab* sl = B > 0 && choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, true, &slab) ? &slab : nullptr;
+  a.chan_stride = C;
+  if (sl) {
+    a.words = (uint64_t*)ws;
+    a.parts = slab.parts;
+    a.chan = (float2*)(a.words + (slab.parts > 1 ? slab_words(a.g, slab) / 2 : 0));
+    a.chan_rows = (int)slab_rows(slab);
+  } else {
+    a.part = (float2*)ws;
+    a.chan = a.part + bwd_part_bytes(a.g, dtype) / sizeof(float2);
+    a.chan_rows = B;
+    a.moments = a.chan + (size_t)B * C;
+  }
   a.dgamma = dgamma; a.dbeta = dbeta; a.ga = ga; a.gb = gb;
-  return dtype == MI_BF16 ? launch_gn_bwd_bf16(a, s) : launch_gn_bwd_f32(a, s);
+  return dtype == MI_BF16 ? launch_gn_bwd_bf16(a, sl, s) : launch_gn_bwd_f32(a, sl, s);
 }
 
 }  // namespace mi

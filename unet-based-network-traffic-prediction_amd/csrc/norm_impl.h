@@ -47,10 +47,12 @@ struct NormArgs {
   int act;
   float eps;
   float2* part;                        // forward: [B][tiles][pieces] float4; backward: [B][tiles][nv * N] (sum dz, sum dz*h)
-  float2* chan;                        // backward: [B][C] (sum dz, sum dz*h) of an image
+  float2* chan;                        // backward: rows of (sum dz, sum dz*h) of each channel, chan_rows of chan_stride
+  int chan_rows, chan_stride;
   float2* moments;                     // backward: [B][G] (mean t, mean t*h)
   float* dgamma; float* dbeta; float ga, gb;
   uint64_t* words;                     // what the parts of an image tell each other
+  int parts;
   DropArgs drop;
 };
 
@@ -273,6 +275,7 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const NormArgs a) {
 //
 // A workgroup owns `nb` images x cv vectors.  Its threads are (image, row, lane): lanes lie along the channels, tpi
 // threads share an image.  A group's sum goes over the rows and lanes of a wave by shuffles and over waves through LDS.
+constexpr int kSlabThreads = 256;
 struct Slab {
   int cv;                      // vectors per pixel of a chunk: whole groups
   int lanes, log_lanes;        // power of two >= cv, at most 64
@@ -343,11 +346,12 @@ template <int I> __device__ __forceinline__ void zero_missing(const SlabPixels& 
 #pragma unroll
   for (int i = 0; i < I; ++i) v[i] = i < px.mine ? v[i] : u32x4_t{0, 0, 0, 0};
 }
-// Ends the lifetime of values unpacked from v: without it the compiler keeps all N * I of them from one use to the next
-// (bf16: twice the registers of v itself) instead of unpacking again.
-template <int I> __device__ __forceinline__ void repack(u32x4_t (&v)[I]) {
-#pragma unroll
-  for (int i = 0; i < I; ++i) asm volatile("" : "+v"(v[i]));
+// Ends the lifetime of what was derived from v: without it the compiler unpacks the vectors of all of a thread's pixels in
+// advance and keeps them (bf16: twice the registers of the vectors) from one use to the next.  `after` is a result that
+// the use has to wait for; WHICH tells branches of one switch apart, whose common beginnings would otherwise move in front
+// of the switch.
+template <int WHICH = -1> __device__ __forceinline__ void pin(u32x4_t& v, float after) {
+  asm volatile("; %1" : "+v"(v) : "n"(WHICH), "v"(after));
 }
 // K sums over each group of each image: in, a thread's K x NS partial sums (of its vector's pieces); out, the sums of the
 // groups that its pieces belong to.  `shared`: as much as slab_shared says; free to use again after a barrier.
@@ -400,49 +404,65 @@ __device__ __forceinline__ void slab_sum(float (&v)[K][NS], const NormGeom& g, c
     }
   }
 }
-// Sum and sum of squares of a thread's vectors, per piece.
-template <int NS, int I>
-__device__ __forceinline__ void power_sums(const u32x4_t (&v)[I], float (&s)[2][NS], float) {
+// Adds a vector to the sums and the sums of squares of its pieces.
+template <int NS> __device__ __forceinline__ void power_sums(u32x4_t v, float (&s)[2][NS], float) {
 #pragma unroll
-  for (int i = 0; i < I; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float f = __uint_as_float(v[i][j]);
-      s[0][j * NS / 4] += f;
-      s[1][j * NS / 4] = fmaf(f, f, s[1][j * NS / 4]);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const float f = __uint_as_float(v[j]);
+    s[0][j * NS / 4] += f;
+    s[1][j * NS / 4] = fmaf(f, f, s[1][j * NS / 4]);
+  }
 }
 // bf16: two products and the sum in one instruction, products exact, accumulated in fp32, nothing to unpack
-template <int NS, int I>
-__device__ __forceinline__ void power_sums(const u32x4_t (&v)[I], float (&s)[2][NS], __bf16) {
+template <int NS> __device__ __forceinline__ void power_sums(u32x4_t v, float (&s)[2][NS], __bf16) {
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int i = 0; i < I; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (NS == 8) {
-        const float lo = __uint_as_float(v[i][j] << 16), hi = __uint_as_float(v[i][j] & 0xffff0000u);
-        s[0][2 * j] += lo;
-        s[0][2 * j + 1] += hi;
-        s[1][2 * j] = fmaf(lo, lo, s[1][2 * j]);
-        s[1][2 * j + 1] = fmaf(hi, hi, s[1][2 * j + 1]);
-      } else {
-        const bf16x2_t x = __builtin_bit_cast(bf16x2_t, (uint32_t)v[i][j]), one = __builtin_bit_cast(bf16x2_t, 0x3f803f80u);
-        s[0][j * NS / 4] = __builtin_amdgcn_fdot2_f32_bf16(x, one, s[0][j * NS / 4], false);
-        s[1][j * NS / 4] = __builtin_amdgcn_fdot2_f32_bf16(x, x, s[1][j * NS / 4], false);
-      }
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (NS == 8) {
+      const float lo = __uint_as_float(v[j] << 16), hi = __uint_as_float(v[j] & 0xffff0000u);
+      s[0][2 * j] += lo;
+      s[0][2 * j + 1] += hi;
+      s[1][2 * j] = fmaf(lo, lo, s[1][2 * j]);
+      s[1][2 * j + 1] = fmaf(hi, hi, s[1][2 * j + 1]);
+    } else {
+      const bf16x2_t x = __builtin_bit_cast(bf16x2_t, (uint32_t)v[j]), one = __builtin_bit_cast(bf16x2_t, 0x3f803f80u);
+      s[0][j * NS / 4] = __builtin_amdgcn_fdot2_f32_bf16(x, one, s[0][j * NS / 4], false);
+      s[1][j * NS / 4] = __builtin_amdgcn_fdot2_f32_bf16(x, x, s[1][j * NS / 4], false);
     }
+  }
+}
+// A part's vectors: from the registers of its own workgroup, or one after the other from memory.
+template <typename T, int I> struct InRegisters {
+  static constexpr int kUnroll = I;
+  u32x4_t (&v)[I];
+  __device__ __forceinline__ u32x4_t operator()(int i, float after) const {
+    pin(v[i], after);
+    return v[i];
+  }
+};
+template <typename T, int I> struct InMemory {
+  static constexpr int kUnroll = 1;
+  const T* first;              // this thread's first pixel and vector
+  int64_t step;
+  int mine;
+  __device__ __forceinline__ u32x4_t operator()(int i, float) const { return i < mine ? load_stream(first + i * step) : u32x4_t{0, 0, 0, 0}; }
+};
+template <typename T, int I>
+__device__ __forceinline__ InMemory<T, I> in_memory(const SlabThread& t, const SlabPixels& px, const NormGeom& g, const Slab& s, const void* base,
+                                                    int cs, int co) {
+  return InMemory<T, I>{(const T*)base + ((int64_t)t.b * g.P + px.first + t.row) * cs + co + t.v * ActVec<T>::N, (int64_t)s.rows * cs, px.mine};
 }
 // Mean (as m + e, m rounded) and squared deviations of the groups over a part.  Sums of x and x^2 first: they do where
 // the deviations are not small against the values, 4 q >= sum x^2 -- what is lost then are two bits.  Groups further from
-// zero take the corrected two-pass form from the registers.  Which of the two is decided for each group by its own values.
-template <typename T, int NS, int I>
-__device__ __forceinline__ void slab_moments(u32x4_t (&v)[I], const SlabPixels& px, const NormGeom& g, const Slab& s, const SlabThread& t,
+// zero take the corrected two-pass form.  Which of the two is decided for each group by its own values.
+template <typename T, int NS, int I, typename V>
+__device__ __forceinline__ void slab_moments(const V& v, const SlabPixels& px, const NormGeom& g, const Slab& s, const SlabThread& t,
                                              float* shared, float* m, float* e, float* q) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   const float n = (float)px.count * (float)g.cg, inv = 1.f / n;
   float sum[2][NS] = {};
-  power_sums<NS, I>(v, sum, T());
+#pragma unroll V::kUnroll
+  for (int i = 0; i < I; ++i) power_sums<NS>(v(i, 0.f), sum, T());
   slab_sum<NS, 2>(sum, g, s, t, shared);
   bool far = false;
 #pragma unroll
@@ -453,12 +473,11 @@ __device__ __forceinline__ void slab_moments(u32x4_t (&v)[I], const SlabPixels& 
     far = far || !(4.f * q[j] >= sum[1][j]);
   }
   if (__syncthreads_or(far && t.live)) {
-    repack(v);
     float dev[2][NS] = {};
-#pragma unroll
+#pragma unroll V::kUnroll
     for (int i = 0; i < I; ++i) {
       float f[N];
-      ActVec<T>::unpack(v[i], f);
+      ActVec<T>::unpack(v(i, m[0]), f);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float d = i < px.mine ? f[j] - m[j / Q] : 0.f;
@@ -478,21 +497,21 @@ __device__ __forceinline__ void slab_moments(u32x4_t (&v)[I], const SlabPixels& 
 }
 
 // ---------------------------------------------------------------- parts of an image
-// Each workgroup of an image publishes its part's sums for the others, two 64-bit words per (image, part, group), and
+// Each workgroup of an image publishes its part's sums for the others, 64-bit words for each (image, part, group), and
 // takes the sums of all parts in one order, so all get the same bits.  A word is valid as soon as it is not kEmpty,
 // which the words are filled with before the launch and which no sum can be: there is nothing else to wait for, and
 // plain device-scope loads and stores do (a release would write the whole L2 back).
 // A part may take long to come -- its workgroup may not run yet, or never at the same time as this one.  No workgroup
-// depends on that: after `polls` looks it forms a missing part's sums itself (the same operations in the same order)
-// and publishes them, so every wait ends.
+// depends on that: after `polls` looks it forms a missing part's sums itself (from memory, the same operations in the same
+// order) and publishes them, so every wait ends.
 constexpr uint64_t kEmpty = ~0ull;
 __device__ __forceinline__ void put_word(uint64_t* p, uint64_t w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ uint64_t get_word(const uint64_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// Runs `take(group of the chunk, present, word 0, word 1)` for every (group, part) of the workgroup's image with lane
-// % 2^log_parts = part, once all parts are there.  Returns the number of a missing part, or -1.
-template <typename F>
+// Runs `take(group of the chunk, present, first word, last word)` for every (group, part) of the workgroup's image, lane
+// % 2^log_parts = part, once all W words of all parts are there.  Returns the number of a missing part, or -1.
+template <int W, typename F>
 __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeom& g, const Slab& s, const SlabThread& t, int groups,
                                             int* missing, F take) {
   const int tid = threadIdx.x, lane = tid & 63, per_wave = 64 >> s.log_parts;
@@ -502,11 +521,11 @@ __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeo
   for (int k = (tid >> 6) * per_wave; k < groups; k += (s.threads >> 6) * per_wave) {
     const int group = k + (lane >> s.log_parts);
     const bool needed = part < s.parts && group < groups;
-    const uint64_t* w = words + 2 * ((int64_t)min(part, s.parts - 1) * g.G + min(group, groups - 1));
+    const uint64_t* w = words + W * ((int64_t)min(part, s.parts - 1) * g.G + min(group, groups - 1));
     uint64_t a = kEmpty, b = kEmpty;
     for (int i = 0;; ++i) {
       a = get_word(w);
-      b = get_word(w + 1);
+      b = W == 2 ? get_word(w + 1) : 0;
       const bool there = !needed || (a != kEmpty && b != kEmpty);
       if (__all(there)) break;
       if (i >= s.polls) {
@@ -532,23 +551,24 @@ __device__ __forceinline__ double parts_total(double v, const Slab& s) {
   return v;
 }
 
-// Two workgroups a CU (128 registers): one loads or stores while the other sums.  (Eight pieces per vector with parts
-// need more; groups of odd channel counts in large images run one workgroup a CU.)
+// 256 threads with up to 16 vectors each: what a thread does once -- its place, its channels' parameters, the sums over
+// other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors: 16.3 us against 16.4
+// for 512 images of 32x32x32 forward, backward with 4 vectors 59 against 32).  128 registers: four workgroups a CU.
 template <typename T, int NS, int I, bool PARTS>
-__global__ __launch_bounds__(512, PARTS && NS > 2 ? 2 : 4) void gn_fwd_slab_kernel(const NormArgs a, const Slab s) {
+__global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_fwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   extern __shared__ float shared[];
   const NormGeom& g = a.g;
   const SlabThread t = slab_thread(g, s);
   const int c0 = t.v * N;
-  SlabPixels px = slab_pixels<I>(t, g, s, t.part);
+  const SlabPixels px = slab_pixels<I>(t, g, s, t.part);
   u32x4_t v[I];
-  load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, v);
   float gamma[N], beta[N];
   if constexpr (!PARTS) {
     load_channels<N>(a.gamma, 1.f, c0, g.C, gamma);
     load_channels<N>(a.beta, 0.f, c0, g.C, beta);
   }
+  load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, v);
   KeepBits<I, N> keep;                                           // while the loads are in flight
   if (a.drop.on) {
     const uint64_t offset = drop_offset(a.drop);
@@ -560,8 +580,8 @@ __global__ __launch_bounds__(512, PARTS && NS > 2 ? 2 : 4) void gn_fwd_slab_kern
   }
   zero_missing(px, v);
   float mean[NS], rstd[NS], e[NS], q[NS];
+  slab_moments<T, NS, I>(InRegisters<T, I>{v}, px, g, s, t, shared, mean, e, q);
   if constexpr (!PARTS) {
-    slab_moments<T, NS, I>(v, px, g, s, t, shared, mean, e, q);
     const float inv = 1.f / ((float)g.P * (float)g.cg);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -573,22 +593,20 @@ __global__ __launch_bounds__(512, PARTS && NS > 2 ? 2 : 4) void gn_fwd_slab_kern
     float* stats = shared + slab_stats_at<NS>(s);                // (mean, rstd) of each group of the chunk, then one int
     const int g0 = t.chunk * s.cv * N / g.cg, groups = min(s.cv * N / g.cg, g.G - g0);
     uint64_t* words = a.words + 2 * ((int64_t)t.b * s.parts * g.G + g0);
-    int part = t.part;
-    for (;;) {
-      slab_moments<T, NS, I>(v, px, g, s, t, shared, mean, e, q);
-      if (t.row == 0 && t.live) {
+    auto publish = [&](int part) {
+      if (t.row != 0 || !t.live) return;
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          const int c = c0 + j * Q, gi = (int)fdiv((uint32_t)min(c, g.C - 1), g.d_cg);
-          if (c == gi * g.cg) {                                  // a group's first piece
-            uint64_t* w = words + 2 * ((int64_t)part * g.G + gi - g0);
-            put_word(w, (uint64_t)__double_as_longlong((double)mean[j] + (double)e[j]));
-            put_word(w + 1, (uint64_t)__double_as_longlong((double)q[j]));
-          }
-        }
+      for (int j = 0; j < NS; ++j) {
+        const int c = c0 + j * Q, gi = (int)fdiv((uint32_t)min(c, g.C - 1), g.d_cg);
+        if (c != gi * g.cg) continue;                            // not a group's first piece
+        uint64_t* w = words + 2 * ((int64_t)part * g.G + gi - g0);
+        put_word(w, (uint64_t)__double_as_longlong((double)mean[j] + (double)e[j]));
+        put_word(w + 1, (uint64_t)__double_as_longlong((double)q[j]));
       }
-      if (part != t.part) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      part = slab_collect(words, g, s, t, groups, (int*)(stats + 2 * groups), [&](int group, bool there, uint64_t w0, uint64_t w1) {
+    };
+    publish(t.part);
+    for (;;) {
+      const int part = slab_collect<2>(words, g, s, t, groups, (int*)(stats + 2 * groups), [&](int group, bool there, uint64_t w0, uint64_t w1) {
         const int p = threadIdx.x & ((1 << s.log_parts) - 1);
         const double n = there ? (double)min(g.P - p * s.rows * I, s.rows * I) * g.cg : 0.0;
         const double m = there ? __longlong_as_double((long long)w0) : 0.0, dev = there ? __longlong_as_double((long long)w1) : 0.0;
@@ -599,16 +617,11 @@ __global__ __launch_bounds__(512, PARTS && NS > 2 ? 2 : 4) void gn_fwd_slab_kern
           stats[2 * group + 1] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)a.eps));
         }
       });
-      if (part < 0) break;
-      px = slab_pixels<I>(t, g, s, part);
-      asm volatile("" : "+v"(px.first));                         // nothing of the addresses is to be kept from the first reading
-      load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, v);
-      zero_missing(px, v);
-    }
-    if (px.first != t.part * s.rows * I) {                       // the registers hold another part: read this one again
-      px = slab_pixels<I>(t, g, s, t.part);
-      asm volatile("" : "+v"(px.first));
-      load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, v);
+      if (__builtin_expect(part < 0, 1)) break;
+      const SlabPixels other = slab_pixels<I>(t, g, s, part);
+      slab_moments<T, NS, I>(in_memory<T, I>(t, other, g, s, a.x, a.xcs, a.xco), other, g, s, t, shared, mean, e, q);
+      publish(part);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // the next look finds it
     }
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -619,7 +632,6 @@ __global__ __launch_bounds__(512, PARTS && NS > 2 ? 2 : 4) void gn_fwd_slab_kern
     load_channels<N>(a.gamma, 1.f, c0, g.C, gamma);              // only now: the exchange needs the registers
     load_channels<N>(a.beta, 0.f, c0, g.C, beta);
   }
-  repack(v);
   if (t.row == 0 && t.live && t.part == 0) {
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -630,23 +642,18 @@ __global__ __launch_bounds__(512, PARTS && NS > 2 ? 2 : 4) void gn_fwd_slab_kern
       }
     }
   }
-  // z = (x - mean) * (rstd * gamma) + beta; in bf16 x * (rstd * gamma) + (beta - mean * rstd * gamma), whose rounding,
-  // 2^-24 of |x| and |mean|, is far below the 2^-9 that x itself was rounded by
-  constexpr bool kOneFma = N == 8;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    gamma[j] *= rstd[j / Q];
-    if (kOneFma) beta[j] = fmaf(-mean[j / Q], gamma[j], beta[j]);
-  }
+  for (int j = 0; j < N; ++j) gamma[j] *= rstd[j / Q];           // z = (x - mean) * (rstd * gamma) + beta
   T* out = (T*)a.out + ((int64_t)t.b * g.P + px.first + t.row) * a.ocs + a.oco + c0;
   const bool tail = c0 + N > g.C;
   auto emit = [&](auto act) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
+      pin<decltype(act)::value>(v[i], rstd[0]);
       float f[N];
       ActVec<T>::unpack(v[i], f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = act_value<decltype(act)::value>(fmaf(kOneFma ? f[j] : f[j] - mean[j / Q], gamma[j], beta[j]));
+      for (int j = 0; j < N; ++j) f[j] = act_value<decltype(act)::value>(fmaf(f[j] - mean[j / Q], gamma[j], beta[j]));
       if (a.drop.on) {
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = keep.kept(i, j, f[j] * a.drop.scale);
@@ -774,9 +781,317 @@ __global__ __launch_bounds__(kThreads) void gn_bwd_apply_kernel(const NormArgs a
     if (w.live && i < w.n) store_stream(out + (int64_t)p * a.ocs, ActVec<T>::pack(dx));
   }
 }
+// h, and z where the activation's slope needs it, of channels e0 .. e0 + 3 of a vector.
+template <int NS, int N, int ACT>
+__device__ __forceinline__ void norm_z(int e0, const float* x, const float* mean, const float* rstd, const float* gamma, const float* beta,
+                                       float* h, float* z) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k = (e0 + j) * NS / N;
+    h[j] = (x[j] - mean[k]) * rstd[k];
+    if (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) z[j] = fmaf(h[j], gamma[e0 + j], beta[e0 + j]);
+  }
+}
+// ReLU's gate is a border that fp32 rounding of z may cross.  But z > 0 is  sign(gamma) x > sign(gamma) tau  with
+// tau = mean - beta / (rstd gamma), and x is an fp32 value: against tau in 64 bits, rounded down to fp32, the comparison is
+// exact.  A channel's tau is worked out once per workgroup; the gate costs two instructions and needs no z.
+__device__ __forceinline__ float relu_threshold(float mean, float rstd, float gamma, float beta) {
+  if (gamma == 0.f) return beta > 0.f ? -INFINITY : INFINITY;
+  double tau = (double)mean - (double)beta / ((double)rstd * (double)gamma);
+  if (gamma < 0.f) tau = -tau;
+  const float f = (float)tau;
+  return (double)f > tau ? nextafterf(f, -INFINITY) : f;
+}
+__device__ __forceinline__ bool relu_gate(float x, float gamma, float threshold) {
+  return __uint_as_float(__builtin_amdgcn_bitop3_b32(__float_as_uint(x), __float_as_uint(gamma), 0x80000000u, 0x78)) > threshold;   // x ^ (gamma & sign)
+}
+// The thresholds of a thread's channels, through LDS (nb * lanes * N floats).  `first` brings a thread's first channel: it is
+// read before the tile's loads are issued, which complete in order.
+struct ReluInputs { float mean, rstd, gamma, beta; };
+__device__ __forceinline__ ReluInputs relu_inputs(const NormArgs& a, const SlabThread& t, int c0, int k) {
+  const int c = min(c0 + k, a.g.C - 1);
+  const int64_t gi = (int64_t)t.b * a.g.G + fdiv((uint32_t)c, a.g.d_cg);
+  return ReluInputs{a.mean[gi], a.rstd[gi], a.gamma ? a.gamma[c] : 1.f, a.beta ? a.beta[c] : 0.f};
+}
+template <int N>
+__device__ __forceinline__ void relu_thresholds(const NormArgs& a, const Slab& s, const SlabThread& t, ReluInputs first, float* shared, float* out) {
+  float* mine = shared + t.slot * s.lanes * N;
+  for (int k = t.tin; k < s.lanes * N; k += s.tpi) {
+    const ReluInputs r = k == t.tin ? first : relu_inputs(a, t, t.chunk * s.cv * N, k);
+    mine[k] = relu_threshold(r.mean, r.rstd, r.gamma, r.beta);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < N; ++j) out[j] = mine[t.lane * N + j];
+  __syncthreads();
+}
+template <int NS, int N>
+__device__ __forceinline__ void slab_channels(const NormArgs& a, int b, int c0, float* mean, float* rstd, float* gamma, float* beta) {
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const int64_t gi = (int64_t)b * a.g.G + fdiv((uint32_t)min(c0 + j * N / NS, a.g.C - 1), a.g.d_cg);
+    mean[j] = a.mean[gi];
+    rstd[j] = a.rstd[gi];
+  }
+  load_channels<N>(a.gamma, 1.f, c0, a.g.C, gamma);
+  load_channels<N>(a.beta, 0.f, c0, a.g.C, beta);
+}
+__device__ __forceinline__ int opaque(int v) {                   // a value whose uses are not prepared in advance
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// Publishes a part's two sums of each group.
+template <int NS, int N>
+__device__ __forceinline__ void publish_bwd(const NormArgs& a, const SlabThread& t, int part, const float (&sum)[2][NS]) {
+  if (t.row != 0 || !t.live) return;
+  const NormGeom& g = a.g;
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const int c = t.v * N + j * (N / NS), gi = (int)fdiv((uint32_t)min(c, g.C - 1), g.d_cg);
+    if (c != gi * g.cg) continue;                                // not a group's first piece
+    const uint32_t w0 = sum[0][j] == sum[0][j] ? __float_as_uint(sum[0][j]) : 0x7fc00000u;   // never kEmpty
+    const uint32_t w1 = sum[1][j] == sum[1][j] ? __float_as_uint(sum[1][j]) : 0x7fc00000u;
+    put_word(a.words + ((int64_t)t.b * a.parts + part) * g.G + gi, (uint64_t)w1 << 32 | w0);
+  }
+}
+// Sums M values over the lanes that differ in bits lanes .. o; every total lands in dst.
+template <int M> __device__ __forceinline__ void scatter_sum(const float* v, int o, int lanes, int lane, float* dst) {
+  if (o < lanes) {
+#pragma unroll
+    for (int j = 0; j < M; ++j) dst[j] = v[j];
+    return;
+  }
+  if constexpr (M > 1) {
+    const bool up = (lane & o) != 0;
+    float r[M / 2];
+#pragma unroll
+    for (int j = 0; j < M / 2; ++j) r[j] = (up ? v[M / 2 + j] : v[j]) + __shfl_xor(up ? v[j] : v[M / 2 + j], o, 64);
+    scatter_sum<M / 2>(r, o >> 1, lanes, lane, dst + (up ? M / 2 : 0));
+  } else {
+    float r = v[0];
+    for (; o >= lanes; o >>= 1) r += __shfl_xor(r, o, 64);
+    dst[0] = r;                                                  // lanes that differ in these bits write the same value
+  }
+}
+// A channel's sums: the gradients themselves if there is one row of them, else a row for gn_param_grads_kernel.
+__device__ __forceinline__ void store_channel(const NormArgs& a, int row, int c, float sum_dz, float sum_dzh) {
+  if (a.chan_rows > 1) {
+    a.chan[(int64_t)row * a.chan_stride + c] = make_float2(sum_dz, sum_dzh);
+    return;
+  }
+  if (a.dgamma) a.dgamma[c] = a.ga * sum_dzh + (a.gb != 0.f ? a.gb * a.dgamma[c] : 0.f);
+  if (a.dbeta) a.dbeta[c] = a.ga * sum_dz + (a.gb != 0.f ? a.gb * a.dbeta[c] : 0.f);
+}
+// Adds a vector's dz and dz * h to the sums of its channels.  What the second pass needs of dy comes back in d: with
+// dropped and gated-off units cleared, in fp32 as dz itself (a bf16 dz would be rounded: its slope is worked out again).
+template <typename T, int NS, int ACT, typename KEEP>
+__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const KEEP& keep, int i, const float* mean, const float* rstd,
+                                         const float* gamma, const float* beta, const float* threshold, float* ch) {
+  constexpr int N = ActVec<T>::N;
+#pragma unroll
+  for (int e = 0; e < N / 4; ++e) {
+    float x[4], d[4], h[4], z[4];
+    ActVec<T>::unpack4(x4, e, x);
+    ActVec<T>::unpack4(d4, e, d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = keep.kept(i, 4 * e + j, d[j]);
+    norm_z<NS, N, ACT>(4 * e, x, mean, rstd, gamma, beta, h, z);
+    if constexpr (ACT == MI_ACT_RELU) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = relu_gate(x[j], gamma[4 * e + j], threshold[4 * e + j]) ? d[j] : 0.f;
+    }
+    if constexpr (N == 8) ActVec<T>::pack4_exact(d, e, d4);
+    if constexpr (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(z[j]);
+    }
+    if constexpr (N == 4) ActVec<T>::pack4(d, e, d4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ch[4 * e + j] += d[j];
+      ch[N + 4 * e + j] = fmaf(d[j], h[j], ch[N + 4 * e + j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);                           // one group after the other: together they need several times the registers
+  }
+}
+// A group's two sums from those of a thread's channels.
+template <int NS, int N> __device__ __forceinline__ void bwd_group_sums(const float* ch, const float* gamma, float (&sum)[2][NS]) {
+#pragma unroll
+  for (int j = 0; j < NS; ++j) sum[0][j] = sum[1][j] = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    sum[0][j * NS / N] = fmaf(gamma[j], ch[j], sum[0][j * NS / N]);
+    sum[1][j * NS / N] = fmaf(gamma[j], ch[N + j], sum[1][j * NS / N]);
+  }
+}
+// The sums of a part whose workgroup has not come, from memory: the same operations in the same order, one vector at a time.
+template <typename T, int NS, int I, int ACT>
+__device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s, const SlabThread& t, int part, float* shared) {
+  constexpr int N = ActVec<T>::N;
+  const NormGeom& g = a.g;
+  const SlabPixels px = slab_pixels<I>(t, g, s, part);
+  const int c0 = opaque(t.v * N), chunk_c0 = t.chunk * s.cv * N;
+  float mean[NS], rstd[NS], gamma[N], beta[N], threshold[N], ch[2 * N] = {}, sum[2][NS];
+  slab_channels<NS, N>(a, t.b, c0, mean, rstd, gamma, beta);
+  if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, relu_inputs(a, t, chunk_c0, t.tin), shared, threshold);
+  const auto x = in_memory<T, I>(t, px, g, s, a.x, a.xcs, a.xco), dy = in_memory<T, I>(t, px, g, s, a.dy, a.ycs, a.yco);
+#pragma unroll 1
+  for (int i = 0; i < I; ++i) {
+    u32x4_t d = dy(i, 0.f);
+    KeepBits<1, N> keep;
+    keep.keep_all();
+    if (a.drop.on) {
+      const uint64_t row = a.drop.per_channel ? (uint64_t)t.b : (uint64_t)t.b * g.P + (px.first + t.row + i * s.rows);
+      keep.add(0, a.drop, drop_offset(a.drop), row * (uint32_t)(g.nv * N) + c0);
+    }
+    bwd_step<T, NS, ACT>(x(i, 0.f), d, keep, 0, mean, rstd, gamma, beta, threshold, ch);
+  }
+  bwd_group_sums<NS, N>(ch, gamma, sum);
+  slab_sum<NS, 2>(sum, g, s, t, shared);
+  publish_bwd<NS, N>(a, t, part, sum);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the next look finds it
+}
+// One read of x and dy: the same division of the work as forward.  Sums of dz and dz * h for each channel come first; a
+// group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
+// linear in it.
+template <typename T, int NS, int I, bool PARTS, int ACT>
+__global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
+  constexpr int N = ActVec<T>::N, Q = N / NS;
+  extern __shared__ float shared[];
+  const NormGeom& g = a.g;
+  const SlabThread t = slab_thread(g, s);
+  const int c0 = t.v * N, chunk_c0 = t.chunk * s.cv * N;
+  const float scale = a.drop.on ? a.drop.scale : 1.f;
+  const SlabPixels px = slab_pixels<I>(t, g, s, t.part);
+  u32x4_t vx[I], vd[I];
+  float mean[NS], rstd[NS], gamma[N], beta[N], threshold[N];
+  float sum[2][NS];                                              // then the means of t and t * h
+  {
+    ReluInputs first;
+    if constexpr (ACT == MI_ACT_RELU) first = relu_inputs(a, t, chunk_c0, t.tin);
+    slab_channels<NS, N>(a, t.b, c0, mean, rstd, gamma, beta);
+    load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, vx);
+    load_slab<T, I>(t, px, g, s, a.dy, a.ycs, a.yco, vd);
+    if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, first, shared, threshold);
+    KeepBits<I, N> keep;                                         // while the loads are in flight
+    if (a.drop.on) {
+      const uint64_t offset = drop_offset(a.drop);
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const uint64_t row = a.drop.per_channel ? (uint64_t)t.b : (uint64_t)t.b * g.P + (px.first + t.row + i * s.rows);
+        keep.add(i, a.drop, offset, row * (uint32_t)(g.nv * N) + c0);
+      }
+    } else {
+      keep.keep_all();                                           // two instructions a value, against branches that cost registers
+    }
+    zero_missing(px, vx);
+    zero_missing(px, vd);
+    float ch[2 * N] = {};                                        // sum dz, sum dz * h of each channel
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      pin(vx[i], rstd[0]);
+      pin(vd[i], rstd[0]);
+      keep.pin();
+      bwd_step<T, NS, ACT>(vx[i], vd[i], keep, i, mean, rstd, gamma, beta, threshold, ch);
+    }
+    bwd_group_sums<NS, N>(ch, gamma, sum);
+    slab_sum<NS, 2>(sum, g, s, t, shared);
+    if constexpr (PARTS) publish_bwd<NS, N>(a, t, t.part, sum);
+    if (a.dgamma != nullptr || a.dbeta != nullptr) {
+      // the workgroup's sums of each channel, over rows and images: lanes first, each stage halves what a lane holds
+      __syncthreads();
+      const int lane = threadIdx.x & 63, waves = s.threads >> 6;
+      if (!t.live) {
+#pragma unroll
+        for (int j = 0; j < 2 * N; ++j) ch[j] = 0.f;
+      }
+      scatter_sum<2 * N>(ch, 32, s.lanes, lane, shared + ((threadIdx.x >> 6) * s.lanes + (lane & (s.lanes - 1))) * (2 * N));
+      __syncthreads();
+      for (int k = threadIdx.x; k < s.lanes * N; k += s.threads) {
+        const int l = k / N, j = k & (N - 1), c = chunk_c0 + k;
+        if (l >= s.cv || c >= g.C) continue;
+        float sa = 0.f, sq = 0.f;
+        for (int w = 0; w < waves; ++w) {
+          sa += shared[(w * s.lanes + l) * 2 * N + j];
+          sq += shared[(w * s.lanes + l) * 2 * N + N + j];
+        }
+        store_channel(a, (int)(blockIdx.x / s.chunks), c, sa * scale, sq * scale);
+      }
+    }
+  }
+  if constexpr (!PARTS) {
+    const float inv = 1.f / ((float)g.P * (float)g.cg);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      sum[0][j] *= inv;
+      sum[1][j] *= inv;
+    }
+  } else {
+    const int g0 = chunk_c0 / g.cg, groups = min(s.cv * N / g.cg, g.G - g0);
+    const uint64_t* words = a.words + ((int64_t)t.b * s.parts * g.G + g0);
+    float* stats = shared + slab_stats_at<NS>(s);
+    __syncthreads();
+    for (;;) {
+      const int part = slab_collect<1>(words, g, s, t, groups, (int*)(stats + 2 * groups), [&](int group, bool there, uint64_t w, uint64_t) {
+        const int p = threadIdx.x & ((1 << s.log_parts) - 1);
+        const double n = (double)g.P * g.cg;
+        const double m1 = parts_total(there ? (double)__uint_as_float((uint32_t)w) : 0.0, s) / n;
+        const double m2 = parts_total(there ? (double)__uint_as_float((uint32_t)(w >> 32)) : 0.0, s) / n;
+        if (p == 0 && there) {
+          stats[2 * group] = (float)m1;
+          stats[2 * group + 1] = (float)m2;
+        }
+      });
+      if (__builtin_expect(part < 0, 1)) break;
+      bwd_other_part<T, NS, I, ACT>(a, s, t, part, shared);
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int gi = (int)fdiv((uint32_t)min(c0 + j * Q, g.C - 1), g.d_cg) - g0;
+      sum[0][j] = stats[2 * gi];
+      sum[1][j] = stats[2 * gi + 1];
+    }
+    slab_channels<NS, N>(a, t.b, opaque(c0), mean, rstd, gamma, beta);   // the exchange needs their registers
+  }
+  T* out = (T*)a.out + ((int64_t)t.b * g.P + px.first + t.row) * a.ocs + a.oco + c0;
+  const bool tail = c0 + N > g.C;
+  float rscale[NS];
+#pragma unroll
+  for (int j = 0; j < NS; ++j) rscale[j] = rstd[j] * scale;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    pin(vx[i], sum[0][0]);
+    pin(vd[i], sum[0][0]);
+#pragma unroll
+    for (int e = 0; e < N / 4; ++e) {
+      float x[4], d[4], h[4], z[4];
+      ActVec<T>::unpack4(vx[i], e, x);
+      ActVec<T>::unpack4(vd[i], e, d);
+      norm_z<NS, N, ACT>(4 * e, x, mean, rstd, gamma, beta, h, z);
+      if constexpr (N == 8 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(z[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma clang fp contract(off)   // t is rounded before the subtraction, as it was in the sum: a group of one value gives exactly zero
+        const int k = (4 * e + j) / Q;
+        const float tj = gamma[4 * e + j] * d[j];
+        d[j] = rscale[k] * fmaf(-h[j], sum[1][k], tj - sum[0][k]);
+      }
+      if (tail) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = c0 + 4 * e + j < g.C ? d[j] : 0.f;
+      }
+      ActVec<T>::pack4(d, e, vd[i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (t.live && i < px.mine) store_stream(out + (int64_t)(i * s.rows) * a.ocs, vd[i]);
+  }
+}
+
 // ---------------------------------------------------------------- launches
 // in norm.hip
-bool choose_slab(const NormGeom& g, int N, Slab* out);
 void launch_gn_empty(uint64_t* words, int64_t n, hipStream_t s);
 void launch_gn_join(const NormArgs& a, hipStream_t s);
 void launch_gn_bwd_join(const NormArgs& a, int padded, hipStream_t s);
@@ -801,22 +1116,21 @@ void launch_fwd_slab(const NormArgs& a, const Slab& sl, hipStream_t s) {
   const int floats = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 : 0);
   const unsigned lds = (unsigned)(floats * sizeof(float));
   if (sl.parts > 1) launch_gn_empty(a.words, slab_words(a.g, sl), s);
-  switch (sl.iters) {
-    case 1: hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, 1, false>), grid, block, lds, s, a, sl); break;
-    case 4: hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, 4, false>), grid, block, lds, s, a, sl); break;
-    default:
-      if (sl.parts == 1) hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, 8, false>), grid, block, lds, s, a, sl);
-      else hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, 8, true>), grid, block, lds, s, a, sl);
-  }
+#define GN_SLAB(I, PARTS) hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, I, PARTS>), grid, block, lds, s, a, sl)
+  if (sl.iters == 1) GN_SLAB(1, false);
+  else if (sl.iters == 4 && sl.parts == 1) GN_SLAB(4, false);
+  else if (sl.iters == 4) GN_SLAB(4, true);
+  else if (sl.parts == 1) GN_SLAB(16, false);
+  else GN_SLAB(16, true);
+#undef GN_SLAB
 }
 
 template <typename T>
-int launch_gn_fwd_t(const NormArgs& a, hipStream_t s) {
-  Slab sl;
-  if (choose_slab(a.g, ActVec<T>::N, &sl)) {
-    if (a.g.n_slots == 1) launch_fwd_slab<T, 1>(a, sl, s);
-    else if (two_pieces<T>(a.g)) launch_fwd_slab<T, ActVec<T>::N / 4>(a, sl, s);
-    else launch_fwd_slab<T, ActVec<T>::N>(a, sl, s);
+int launch_gn_fwd_t(const NormArgs& a, const Slab* sl, hipStream_t s) {
+  if (sl != nullptr) {
+    if (a.g.n_slots == 1) launch_fwd_slab<T, 1>(a, *sl, s);
+    else if (two_pieces<T>(a.g)) launch_fwd_slab<T, ActVec<T>::N / 4>(a, *sl, s);
+    else launch_fwd_slab<T, ActVec<T>::N>(a, *sl, s);
     return check_hip(hipGetLastError(), "group_norm_act_fwd");
   }
   const dim3 grid((unsigned)(a.g.B * a.g.tiles * a.g.chunks)), block(kThreads);
@@ -829,8 +1143,39 @@ int launch_gn_fwd_t(const NormArgs& a, hipStream_t s) {
 #undef GN_APPLY
   return check_hip(hipGetLastError(), "group_norm_act_fwd");
 }
+template <typename T, int NS, int ACT>
+void launch_bwd_slab_act(const NormArgs& a, const Slab& sl, dim3 grid, dim3 block, unsigned lds, hipStream_t s) {
+#define GN_SLAB(I, PARTS) hipLaunchKernelGGL((gn_bwd_slab_kernel<T, NS, I, PARTS, ACT>), grid, block, lds, s, a, sl)
+  if (sl.iters == 1) GN_SLAB(1, false);
+  else if (sl.iters == 4 && sl.parts == 1) GN_SLAB(4, false);
+  else if (sl.iters == 4) GN_SLAB(4, true);
+  else if (sl.parts == 1) GN_SLAB(8, false);
+  else GN_SLAB(8, true);
+#undef GN_SLAB
+}
+template <typename T, int NS>
+void launch_bwd_slab(const NormArgs& a, const Slab& sl, hipStream_t s) {
+  const dim3 grid(slab_grid(sl)), block((unsigned)sl.threads);
+  const int sums = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 : 0);
+  const int channels = a.dgamma || a.dbeta ? (sl.threads >> 6) * sl.lanes * 2 * ActVec<T>::N : 0;
+  const int thresholds = a.act == MI_ACT_RELU ? (sl.threads >> sl.log_tpi) * sl.lanes * ActVec<T>::N : 0;
+  int floats = sums > channels ? sums : channels;
+  if (thresholds > floats) floats = thresholds;
+  const unsigned lds = (unsigned)(floats * sizeof(float));
+  if (sl.parts > 1) launch_gn_empty(a.words, slab_words(a.g, sl) / 2, s);
+#define GN_SLAB(A) launch_bwd_slab_act<T, NS, A>(a, sl, grid, block, lds, s)
+  MI_FOR_ACT(a.act, GN_SLAB)
+#undef GN_SLAB
+}
 template <typename T>
-int launch_gn_bwd_t(const NormArgs& a, hipStream_t s) {
+int launch_gn_bwd_t(const NormArgs& a, const Slab* sl, hipStream_t s) {
+  if (sl != nullptr) {
+    if (a.g.n_slots == 1) launch_bwd_slab<T, 1>(a, *sl, s);
+    else if (two_pieces<T>(a.g)) launch_bwd_slab<T, ActVec<T>::N / 4>(a, *sl, s);
+    else launch_bwd_slab<T, ActVec<T>::N>(a, *sl, s);
+    if (a.chan_rows > 1 && (a.dgamma || a.dbeta)) launch_gn_param_grads(a, s);
+    return check_hip(hipGetLastError(), "group_norm_act_bwd");
+  }
   if (a.g.B > 0) {
     const dim3 grid((unsigned)(a.g.B * a.g.tiles * a.g.chunks)), block(kThreads);
 #define GN_SUMS(A) hipLaunchKernelGGL((gn_bwd_sums_kernel<T, A>), grid, block, 0, s, a)
