@@ -68,16 +68,19 @@ struct KeepBits {
       if (at % 16 == 15 || at == kWords - 1) asm("" : "+v"(r[at / 16]));
     }
   }
-  // f where unit j of vector i survives, +0 where it does not
-  __device__ __forceinline__ float kept(int i, int j, float f) const {
+  // all ones where unit j of vector i survives, else zero
+  __device__ __forceinline__ uint32_t mask(int i, int j) const {
     const int at = i * (N / 2) + j / 2, in_reg = at / 16 < kRegs - 1 ? 16 : kWords - 16 * (kRegs - 1);
     const int bit = (j & 1) * 16 + 16 - in_reg + at % 16;
-    return __uint_as_float(__float_as_uint(f) & (uint32_t)((int32_t)(r[at / 16] << (31 - bit)) >> 31));
+    return (uint32_t)((int32_t)(r[at / 16] << (31 - bit)) >> 31);
   }
-  // no bit is looked at before this point
-  __device__ __forceinline__ void pin() {
+  // f where the unit survives, +0 where it does not
+  __device__ __forceinline__ float kept(int i, int j, float f) const { return __uint_as_float(__float_as_uint(f) & mask(i, j)); }
+  // the same for a whole vector of the stored type
+  __device__ __forceinline__ u32x4_t kept(int i, u32x4_t v) const {
 #pragma unroll
-    for (int k = 0; k < kRegs; ++k) asm volatile("" : "+v"(r[k]));
+    for (int h = 0; h < 4; ++h) v[h] &= N == 8 ? __builtin_amdgcn_perm(mask(i, 2 * h + 1), mask(i, 2 * h), 0x05040100) : mask(i, h);
+    return v;
   }
   __device__ __forceinline__ void keep_all() {
 #pragma unroll

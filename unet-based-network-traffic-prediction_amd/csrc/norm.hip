@@ -153,7 +153,7 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   s.chunks = (int)((g.nv + cv - 1) / cv);
   const int64_t vectors = (int64_t)g.P * s.lanes;
   // as many vectors a thread as its registers hold where that leaves every CU a workgroup, else 4: less time for each
-  const int most = backward ? 8 : 16;
+  const int most = 16;
   s.iters = vectors <= s.lanes ? 1 : ((int64_t)g.B * s.chunks * vectors < 256 * most * kSlabThreads ? 4 : most);
   s.tpi = vectors < (int64_t)s.iters * kSlabThreads ? pow2_ceil((vectors + s.iters - 1) / s.iters) : kSlabThreads;
   if (s.tpi < s.lanes) s.tpi = s.lanes;

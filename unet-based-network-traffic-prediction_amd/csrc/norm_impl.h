@@ -882,30 +882,29 @@ __device__ __forceinline__ void store_channel(const NormArgs& a, int row, int c,
   if (a.dgamma) a.dgamma[c] = a.ga * sum_dzh + (a.gb != 0.f ? a.gb * a.dgamma[c] : 0.f);
   if (a.dbeta) a.dbeta[c] = a.ga * sum_dz + (a.gb != 0.f ? a.gb * a.dbeta[c] : 0.f);
 }
-// Adds a vector's dz and dz * h to the sums of its channels.  What the second pass needs of dy comes back in d: with
-// dropped and gated-off units cleared, in fp32 as dz itself (a bf16 dz would be rounded: its slope is worked out again).
-template <typename T, int NS, int ACT, typename KEEP>
-__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const KEEP& keep, int i, const float* mean, const float* rstd,
-                                         const float* gamma, const float* beta, const float* threshold, float* ch) {
+// Adds a vector's dz and dz * h to the sums of its channels (d4: dy, dropped units cleared).  What the second pass needs of
+// dy comes back: with gated-off units cleared, in fp32 as dz itself (a bf16 dz would be rounded: its slope is worked out again).
+template <typename T, int NS, int ACT>
+__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const float* mean, const float* rstd, const float* gamma,
+                                         const float* beta, const float* threshold, float* ch) {
   constexpr int N = ActVec<T>::N;
 #pragma unroll
   for (int e = 0; e < N / 4; ++e) {
     float x[4], d[4], h[4], z[4];
     ActVec<T>::unpack4(x4, e, x);
     ActVec<T>::unpack4(d4, e, d);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = keep.kept(i, 4 * e + j, d[j]);
     norm_z<NS, N, ACT>(4 * e, x, mean, rstd, gamma, beta, h, z);
     if constexpr (ACT == MI_ACT_RELU) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = relu_gate(x[j], gamma[4 * e + j], threshold[4 * e + j]) ? d[j] : 0.f;
+      ActVec<T>::pack4_exact(d, e, d4);
+      if (e == N / 4 - 1) pin(d4, rstd[0]);                      // what was packed is not kept unpacked besides
     }
-    if constexpr (N == 8) ActVec<T>::pack4_exact(d, e, d4);
     if constexpr (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(z[j]);
     }
-    if constexpr (N == 4) ActVec<T>::pack4(d, e, d4);
+    if constexpr (N == 4 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) ActVec<T>::pack4(d, e, d4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       ch[4 * e + j] += d[j];
@@ -938,13 +937,13 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
 #pragma unroll 1
   for (int i = 0; i < I; ++i) {
     u32x4_t d = dy(i, 0.f);
-    KeepBits<1, N> keep;
-    keep.keep_all();
     if (a.drop.on) {
+      KeepBits<1, N> keep;
       const uint64_t row = a.drop.per_channel ? (uint64_t)t.b : (uint64_t)t.b * g.P + (px.first + t.row + i * s.rows);
       keep.add(0, a.drop, drop_offset(a.drop), row * (uint32_t)(g.nv * N) + c0);
+      d = keep.kept(0, d);
     }
-    bwd_step<T, NS, ACT>(x(i, 0.f), d, keep, 0, mean, rstd, gamma, beta, threshold, ch);
+    bwd_step<T, NS, ACT>(x(i, 0.f), d, mean, rstd, gamma, beta, threshold, ch);
   }
   bwd_group_sums<NS, N>(ch, gamma, sum);
   slab_sum<NS, 2>(sum, g, s, t, shared);
@@ -955,7 +954,7 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
 // group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
 // linear in it.
 template <typename T, int NS, int I, bool PARTS, int ACT>
-__global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
+__global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   extern __shared__ float shared[];
   const NormGeom& g = a.g;
@@ -973,16 +972,16 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_bwd_slab_kerne
     load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, vx);
     load_slab<T, I>(t, px, g, s, a.dy, a.ycs, a.yco, vd);
     if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, first, shared, threshold);
-    KeepBits<I, N> keep;                                         // while the loads are in flight
     if (a.drop.on) {
+      KeepBits<I, N> keep;                                       // while the loads are in flight
       const uint64_t offset = drop_offset(a.drop);
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const uint64_t row = a.drop.per_channel ? (uint64_t)t.b : (uint64_t)t.b * g.P + (px.first + t.row + i * s.rows);
         keep.add(i, a.drop, offset, row * (uint32_t)(g.nv * N) + c0);
       }
-    } else {
-      keep.keep_all();                                           // two instructions a value, against branches that cost registers
+#pragma unroll
+      for (int i = 0; i < I; ++i) vd[i] = keep.kept(i, vd[i]);
     }
     zero_missing(px, vx);
     zero_missing(px, vd);
@@ -991,8 +990,7 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_bwd_slab_kerne
     for (int i = 0; i < I; ++i) {
       pin(vx[i], rstd[0]);
       pin(vd[i], rstd[0]);
-      keep.pin();
-      bwd_step<T, NS, ACT>(vx[i], vd[i], keep, i, mean, rstd, gamma, beta, threshold, ch);
+      bwd_step<T, NS, ACT>(vx[i], vd[i], mean, rstd, gamma, beta, threshold, ch);
     }
     bwd_group_sums<NS, N>(ch, gamma, sum);
     slab_sum<NS, 2>(sum, g, s, t, shared);
@@ -1149,8 +1147,8 @@ void launch_bwd_slab_act(const NormArgs& a, const Slab& sl, dim3 grid, dim3 bloc
   if (sl.iters == 1) GN_SLAB(1, false);
   else if (sl.iters == 4 && sl.parts == 1) GN_SLAB(4, false);
   else if (sl.iters == 4) GN_SLAB(4, true);
-  else if (sl.parts == 1) GN_SLAB(8, false);
-  else GN_SLAB(8, true);
+  else if (sl.parts == 1) GN_SLAB(16, false);
+  else GN_SLAB(16, true);
 #undef GN_SLAB
 }
 template <typename T, int NS>
