@@ -198,7 +198,7 @@ int mi_dropout_fwd(const void* x, int x_cstride, int x_coff, const void* residua
 /* y = dropout(act((x - mean) * rstd * gamma + beta)): torch's nn.GroupNorm(groups, C, eps), an activation and a
  * dropout (drop may be NULL) in one operator.  gamma, beta: C floats each, or NULL (1 and 0).  mean, rstd
  * (B*groups floats each) are written; the backward pass reads them.  C must be a multiple of groups.  y must not
- * overlap x.  ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content. */
+ * overlap x.  ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content (NULL where that is 0). */
 int mi_group_norm_act_fwd(const void* x, int x_cstride, int x_coff, const float* gamma, const float* beta,
                           void* y, int y_cstride, int y_coff, float* mean, float* rstd,
                           int B, int H, int W, int C, int groups, int act, float eps, const mi_dropout* drop,

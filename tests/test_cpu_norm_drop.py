@@ -100,8 +100,8 @@ def test_c_refusals(ua):
     for i, call in enumerate(calls):
         assert call() == -1, i                                    # MI_EINVAL
         assert L.mi_last_error().decode()
-    assert _norm_fwd(L, ws_bytes=8) == -2 and b"workspace" in L.mi_last_error()       # MI_ESIZE
-    assert _norm_bwd(L, ws_bytes=8) == -2 and b"workspace" in L.mi_last_error()
+    assert _norm_fwd(L, y=A << 10, B=2, H=400, W=400, ws_bytes=8) == -2 and b"workspace" in L.mi_last_error()       # MI_ESIZE
+    assert _norm_bwd(L, dy=A << 9, dx=A << 10, B=300, H=40, W=40, ws_bytes=8) == -2 and b"workspace" in L.mi_last_error()
 
 
 def test_empty_batches_need_nothing(ua):

@@ -594,8 +594,8 @@ size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backwa
   MI_NHWC_SHAPE(what);                                                                                                   \
   MI_REQUIRE(groups > 0 && C % groups == 0, what ": the channel count must be a multiple of the group count");           \
   MI_REQUIRE(act >= MI_ACT_NONE && act <= MI_ACT_GELU, what ": unknown activation");                                     \
-  MI_REQUIRE(B == 0 || (mean != nullptr && rstd != nullptr && ws != nullptr && ((uintptr_t)ws & 15) == 0),               \
-             what ": statistics or workspace missing or unaligned")
+  MI_REQUIRE(B == 0 || (mean != nullptr && rstd != nullptr), what ": statistics missing");                               \
+  MI_REQUIRE(B == 0 || ((ws != nullptr || ws_bytes == 0) && ((uintptr_t)ws & 15) == 0), what ": workspace missing or unaligned")
 int mi_group_norm_act_fwd(const void* x, int xcs, int xco, const float* gamma, const float* beta, void* y, int ycs, int yco,
                           float* mean, float* rstd, int B, int H, int W, int C, int groups, int act, float eps,
                           const mi_dropout* drop, void* ws, size_t ws_bytes, int dtype, mi_stream s) {

@@ -152,10 +152,16 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   while ((1 << s.log_lanes) < s.lanes) ++s.log_lanes;
   s.chunks = (int)((g.nv + cv - 1) / cv);
   const int64_t vectors = (int64_t)g.P * s.lanes;
-  // as many vectors a thread as its registers hold where that leaves every CU a workgroup, else 4: less time for each
-  const int most = 16;
-  s.iters = vectors <= s.lanes ? 1 : ((int64_t)g.B * s.chunks * vectors < 256 * most * kSlabThreads ? 4 : most);
-  s.tpi = vectors < (int64_t)s.iters * kSlabThreads ? pow2_ceil((vectors + s.iters - 1) / s.iters) : kSlabThreads;
+  // Up to 16 vectors a thread, as many as its registers hold, where that leaves every CU a workgroup.  Else 4, for a
+  // shorter time -- but not where that alone would split an image (parts cost a launch) or, backward, keep the images of
+  // a chunk from sharing a workgroup, which then needs no launch to join the parameter gradients.
+  const int64_t most = 16 * kSlabThreads, few = 4 * kSlabThreads;
+  const bool alone = backward && g.B <= kSlabThreads && pow2_ceil(g.B) * vectors <= most;
+  if (vectors <= s.lanes) s.iters = 1;
+  else if (alone) s.iters = pow2_ceil(g.B) * vectors <= few ? 4 : 16;
+  else if (vectors <= few) s.iters = (int64_t)g.B * s.chunks * vectors < 256 * most ? 4 : 16;
+  else s.iters = vectors > most && (int64_t)g.B * s.chunks * vectors < 256 * most ? 4 : 16;
+  s.tpi = vectors < s.iters * kSlabThreads ? pow2_ceil((vectors + s.iters - 1) / s.iters) : kSlabThreads;
   if (s.tpi < s.lanes) s.tpi = s.lanes;
   while ((1 << s.log_tpi) < s.tpi) ++s.log_tpi;
   s.rows = s.tpi / s.lanes;
@@ -189,11 +195,11 @@ size_t group_norm_ws_bytes(int B, int H, int W, int C, int G, int backward, int 
   const int N = dtype == MI_BF16 ? 8 : 4;
   Slab s;
   if (!backward) {
-    if (choose_slab(g, N, false, &s)) return s.parts > 1 ? slab_words(g, s) * sizeof(uint64_t) : 16;
-    return fwd_part_bytes(g) + 16;
+    if (choose_slab(g, N, false, &s)) return s.parts > 1 ? slab_words(g, s) * sizeof(uint64_t) : 0;
+    return fwd_part_bytes(g);
   }
-  if (choose_slab(g, N, true, &s)) return (s.parts > 1 ? slab_words(g, s) / 2 * sizeof(uint64_t) : 0) + slab_rows(s) * C * sizeof(float2) + 16;
-  return bwd_part_bytes(g, dtype) + ((size_t)B * C + (size_t)B * G) * sizeof(float2) + 16;
+  if (choose_slab(g, N, true, &s)) return (s.parts > 1 ? slab_words(g, s) / 2 * sizeof(uint64_t) : 0) + (slab_rows(s) > 1 ? slab_rows(s) * C * sizeof(float2) : 0);
+  return bwd_part_bytes(g, dtype) + ((size_t)B * C + (size_t)B * G) * sizeof(float2);
 }
 
 static int check_range(const NormGeom& g, const char* what) {

@@ -295,24 +295,36 @@ def _norm_ws_bytes(B, H, W, Cc, groups, backward, dt) -> int:
     return lib().mi_group_norm_ws_bytes(B, H, W, Cc, groups, backward, dt)
 
 
+def _new_activation(x: torch.Tensor, C: int) -> torch.Tensor:
+    """An activation of C channels with the size, type and device of ``x``."""
+    B, H, W, cs = x.shape
+    width = pad_ch(C)
+    return torch.empty_like(x) if width == cs else x.new_empty((B, H, W, width))
+
+
+# The small calls of these layers are bound by the host: ``torch.cuda.current_stream`` builds an object (1.8 us), this
+# returns the handle alone (0.1 us).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def dropout_fwd(x, C, drop: Optional[Drop], residual=None, x_coff=0, residual_coff=0, out=None, out_coff=0):
     """``residual + dropout(x)`` (NHWC, C of the channels from ``x_coff`` on); ``out`` may be x or the residual;
     without a ``drop`` nothing is dropped."""
     _nhwc(x, "dropout")
     B, H, W, cs = x.shape
-    dev = x.device
-    rv = (None, 0, 0)
-    if residual is not None:
+    dev, dt = x.device, mi_dtype(x.dtype)
+    if residual is None:
+        rp, rcs = None, 0
+    else:
         _nhwc(residual, "dropout residual", x)
-        rv = (residual.data_ptr(), residual.shape[3], residual_coff)
+        rp, rcs = residual.data_ptr(), residual.shape[3]
     with _on(dev):
         if out is None:
-            out = torch.empty((B, H, W, pad_ch(C)), device=dev, dtype=x.dtype)
+            out = _new_activation(x, C)
         else:
             _nhwc(out, "dropout out", x)
-        check(lib().mi_dropout_fwd(x.data_ptr(), cs, x_coff, *rv, out.data_ptr(), out.shape[3], out_coff, B, H, W, C,
-                                   _drop_ref(drop, dev), mi_dtype(x.dtype), torch.cuda.current_stream(dev).cuda_stream),
-              "dropout_fwd")
+        check(lib().mi_dropout_fwd(x.data_ptr(), cs, x_coff, rp, rcs, residual_coff, out.data_ptr(), out.shape[3], out_coff, B, H, W,
+                                   C, _drop_ref(drop, dev), dt, _raw_stream(dev.index)), "dropout_fwd")
     return out
 
 
@@ -334,17 +346,16 @@ def group_norm_act_fwd(x, C, groups, weight=None, bias=None, act="none", eps=1e-
         raise ValueError(f"group_norm_act: {C} channels do not split into {groups} groups")
     with _on(dev):
         if out is None:
-            out = torch.empty((B, H, W, pad_ch(C)), device=dev, dtype=x.dtype)
+            out = _new_activation(x, C)
         else:
             _nhwc(out, "group_norm_act out", x)
-        stats = torch.empty((2, B, groups), device=dev, dtype=torch.float32)
+        mean, rstd = torch.empty((2, B, groups), device=dev, dtype=torch.float32).unbind()
         nbytes = _norm_ws_bytes(B, H, W, C, groups, 0, dt)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        sp = stats.data_ptr()
-        check(lib().mi_group_norm_act_fwd(x.data_ptr(), cs, x_coff, wp, bp, out.data_ptr(), out.shape[3], out_coff, sp,
-                                          sp + 4 * B * groups, B, H, W, C, groups, code, eps, _drop_ref(drop, dev), ws.data_ptr(),
-                                          nbytes, dt, torch.cuda.current_stream(dev).cuda_stream), "group_norm_act_fwd")
-    return out, stats[0], stats[1]
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+        check(lib().mi_group_norm_act_fwd(x.data_ptr(), cs, x_coff, wp, bp, out.data_ptr(), out.shape[3], out_coff, mean.data_ptr(),
+                                          rstd.data_ptr(), B, H, W, C, groups, code, eps, _drop_ref(drop, dev),
+                                          ws.data_ptr() if nbytes else None, nbytes, dt, _raw_stream(dev.index)), "group_norm_act_fwd")
+    return out, mean, rstd
 
 
 def group_norm_act_bwd(x, dy, mean, rstd, C, groups, weight=None, bias=None, act="none", drop: Optional[Drop] = None, x_coff=0,
@@ -361,18 +372,18 @@ def group_norm_act_bwd(x, dy, mean, rstd, C, groups, weight=None, bias=None, act
         raise ValueError(f"group_norm_act: {C} channels do not split into {groups} groups")
     mp, rp = (_channel_vector(t, B * groups, dev, "group_norm_act statistics") for t in (mean, rstd))
     with _on(dev):
-        dx = torch.empty((B, H, W, pad_ch(C)), device=dev, dtype=x.dtype)
+        dx = _new_activation(x, C)
         if weight is not None and dweight is None:
             dweight = torch.empty_like(weight) if beta == 0.0 else torch.zeros_like(weight)
         if bias is not None and dbias is None:
             dbias = torch.empty_like(bias) if beta == 0.0 else torch.zeros_like(bias)
         gp, hp = _channel_vector(dweight, C, dev, "group_norm_act dweight"), _channel_vector(dbias, C, dev, "group_norm_act dbias")
         nbytes = _norm_ws_bytes(B, H, W, C, groups, 1, dt)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
         check(lib().mi_group_norm_act_bwd(x.data_ptr(), cs, x_coff, dy.data_ptr(), dy.shape[3], dy_coff, wp, bp, mp, rp,
                                           dx.data_ptr(), dx.shape[3], 0, gp, hp, alpha, beta, B, H, W, C, groups, code,
-                                          _drop_ref(drop, dev), ws.data_ptr(), nbytes, dt,
-                                          torch.cuda.current_stream(dev).cuda_stream), "group_norm_act_bwd")
+                                          _drop_ref(drop, dev), ws.data_ptr() if nbytes else None, nbytes, dt,
+                                          _raw_stream(dev.index)), "group_norm_act_bwd")
     return dx, dweight, dbias
 
 
