@@ -142,8 +142,10 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   Slab s{};
   int64_t cv = g.nv <= 64 ? g.nv : unit * (64 / unit);
   // fewer workgroups than CUs: narrower chunks, down to one line of 128 bytes per pixel
+  const bool small = (int64_t)g.B * g.P * g.nv < 256 * 16 * kSlabThreads;
   for (;;) {
     const int64_t half = cv / 2 / unit * unit, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
+    if (half >= 1 && small && (int64_t)g.P * pow2_ceil(cv) > 16 * kSlabThreads) { cv = half; continue; }
     if (half < 8 || wgs >= 256 || (int64_t)g.P * pow2_ceil(cv) <= 256) break;
     cv = half;
   }
