@@ -136,55 +136,66 @@ static int pow2_ceil(int64_t v) {
 // How the slab kernels divide the work, or false where they do not apply.
 constexpr int kMaxParts = 64;                // lanes of the wave that joins them
 constexpr int kPolls = 4096;
-static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
-  const int unit = g.cg / gcd_int(g.cg, N) < g.nv ? g.cg / gcd_int(g.cg, N) : g.nv;   // vectors after which a group ends with a vector
-  if (unit > 64) return false;
+// The division with `iters` vectors a thread of chunks of cv vectors.
+static bool divide_slab(const NormGeom& g, int64_t cv, int iters, Slab* out) {
   Slab s{};
-  int64_t cv = g.nv <= 64 ? g.nv : unit * (64 / unit);
-  // fewer workgroups than CUs: narrower chunks, down to one line of 128 bytes per pixel
-  const bool small = (int64_t)g.B * g.P * g.nv < 256 * 16 * kSlabThreads;
-  for (;;) {
-    const int64_t half = cv / 2 / unit * unit, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
-    if (half >= 1 && small && (int64_t)g.P * pow2_ceil(cv) > 16 * kSlabThreads) { cv = half; continue; }
-    if (half < 8 || wgs >= 256 || (int64_t)g.P * pow2_ceil(cv) <= 256) break;
-    cv = half;
-  }
+  s.iters = iters;
   s.cv = (int)cv;
   s.lanes = pow2_ceil(cv);
   while ((1 << s.log_lanes) < s.lanes) ++s.log_lanes;
   s.chunks = (int)((g.nv + cv - 1) / cv);
   const int64_t vectors = (int64_t)g.P * s.lanes;
-  // Up to 16 vectors a thread, as many as its registers hold, where that leaves every CU a workgroup.  Else 4, for a
-  // shorter time -- but not where that alone would split an image (parts cost a launch) or, backward, keep the images of
-  // a chunk from sharing a workgroup, which then needs no launch to join the parameter gradients.
-  const int64_t most = 16 * kSlabThreads, few = 4 * kSlabThreads;
-  const bool alone = backward && g.B <= kSlabThreads && pow2_ceil(g.B) * vectors <= most;
-  if (vectors <= s.lanes) s.iters = 1;
-  else if (alone) s.iters = pow2_ceil(g.B) * vectors <= few ? 4 : 16;
-  else if (vectors <= few) s.iters = (int64_t)g.B * s.chunks * vectors < 256 * most ? 4 : 16;
-  else s.iters = vectors > most && (int64_t)g.B * s.chunks * vectors < 256 * most ? 4 : 16;
-  s.tpi = vectors < s.iters * kSlabThreads ? pow2_ceil((vectors + s.iters - 1) / s.iters) : kSlabThreads;
+  s.tpi = vectors < iters * kSlabThreads ? pow2_ceil((vectors + iters - 1) / iters) : kSlabThreads;
   if (s.tpi < s.lanes) s.tpi = s.lanes;
   while ((1 << s.log_tpi) < s.tpi) ++s.log_tpi;
   s.rows = s.tpi / s.lanes;
-  const int64_t parts = (g.P + (int64_t)s.rows * s.iters - 1) / ((int64_t)s.rows * s.iters);
+  const int64_t parts = (g.P + (int64_t)s.rows * iters - 1) / ((int64_t)s.rows * iters);
   if (parts > kMaxParts) return false;
   s.parts = (int)parts;
   while ((1 << s.log_parts) < s.parts) ++s.log_parts;
   s.nb = 1;
-  if (s.parts == 1) {
+  if (s.parts == 1)
     while (s.nb * s.tpi < kSlabThreads && s.nb < g.B) s.nb *= 2;
-  }
   s.img_blocks = (g.B + s.nb - 1) / s.nb;
   s.threads = s.nb * s.tpi < 64 ? 64 : s.nb * s.tpi;
   const int ppg = g.cg / g.q;
   s.merge = g.n_slots == 1 && (ppg & (ppg - 1)) == 0 ? ppg : 1;
   s.left = ppg / s.merge;
-  s.by_xcd = s.chunks > 1 && s.cv < 8 && s.parts == 1 && s.img_blocks >= 8;
   s.polls = kPolls;
   s.d_chunks = make_fastdiv(s.chunks);
   s.d_parts = make_fastdiv(s.parts);
   *out = s;
+  return true;
+}
+static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
+  const int unit = g.cg / gcd_int(g.cg, N) < g.nv ? g.cg / gcd_int(g.cg, N) : g.nv;   // vectors after which a group ends with a vector
+  if (unit > 64) return false;
+  const int64_t most = 16 * kSlabThreads, few = 4 * kSlabThreads;
+  const bool small = (int64_t)g.B * g.P * g.nv < 256 * most;     // not enough to give every CU a full workgroup
+  int64_t cv = g.nv <= 64 ? g.nv : unit * (64 / unit);
+  // fewer workgroups than CUs: narrower chunks, down to one line of 128 bytes per pixel
+  for (;;) {
+    const int64_t half = cv / 2 / unit * unit, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
+    if (half < 8 || wgs >= 256 || g.P * (int64_t)pow2_ceil(cv) <= 256) break;
+    cv = half;
+  }
+  // and below that, to two lanes' width or one, where it spares an image parts (and a launch)
+  if (small && g.P * (int64_t)pow2_ceil(cv) > most) {
+    int64_t narrow = cv;
+    while (narrow >= unit && g.P * (int64_t)pow2_ceil(narrow) > most) narrow = narrow / 2 / unit * unit;
+    if (narrow >= unit) cv = narrow;
+  }
+  const int64_t vectors = (int64_t)g.P * pow2_ceil(cv);
+  // Up to 16 vectors a thread, as many as its registers hold, where that leaves every CU a workgroup.  Else 4, for a
+  // shorter time -- but not where that alone would split an image (parts cost a launch) or, backward, keep the images of
+  // a chunk from sharing a workgroup, which then needs no launch to join the parameter gradients.
+  const bool alone = backward && g.B <= kSlabThreads && pow2_ceil(g.B) * vectors <= most;
+  int iters = small ? 4 : 16;
+  if (vectors <= pow2_ceil(cv)) iters = 1;
+  else if (alone) iters = pow2_ceil(g.B) * vectors <= few ? 4 : 16;
+  else if (vectors > few && vectors <= most) iters = 16;
+  if (!divide_slab(g, cv, iters, out)) return false;
+  out->by_xcd = out->chunks > 1 && out->cv < 8 && out->parts == 1 && out->img_blocks >= 8;
   return true;
 }
 static size_t slab_rows(const Slab& s) { return (size_t)s.img_blocks * s.parts; }   // rows of channel sums

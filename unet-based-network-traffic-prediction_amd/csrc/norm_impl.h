@@ -296,30 +296,32 @@ struct SlabThread {
   int b, v, part, chunk;       // image, vector
   bool live;
 };
+// This thread's place in workgroup `item` of a chunk: (images, part) in the order of memory.
+__device__ __forceinline__ void slab_item(const NormGeom& g, const Slab& s, uint32_t item, SlabThread& t) {
+  const uint32_t ib = fdiv(item, s.d_parts);
+  t.part = (int)(item - ib * s.parts);
+  t.b = (int)ib * s.nb + t.slot;
+  t.live = t.slot < s.nb && t.b < g.B && t.lane < s.cv && t.chunk * s.cv + t.lane < g.nv;
+  t.b = min(t.b, g.B - 1);
+}
 __device__ __forceinline__ SlabThread slab_thread(const NormGeom& g, const Slab& s) {
   SlabThread t;
-  uint32_t i = blockIdx.x, ib;
+  uint32_t item;
   if (s.by_xcd) {                                                // workgroup i runs on XCD i % 8
-    const uint32_t j = i >> 3, q = fdiv(j, s.d_chunks);
+    const uint32_t i = blockIdx.x, j = i >> 3, q = fdiv(j, s.d_chunks);
     t.chunk = (int)(j - q * s.chunks);
-    ib = q * 8 + (i & 7);
-    t.part = 0;
+    item = q * 8 + (i & 7);
   } else {
-    const uint32_t q = fdiv(i, s.d_chunks);
-    t.chunk = (int)(i - q * s.chunks);
-    ib = fdiv(q, s.d_parts);
-    t.part = (int)(q - ib * s.parts);
+    item = fdiv(blockIdx.x, s.d_chunks);
+    t.chunk = (int)(blockIdx.x - item * s.chunks);
   }
   const int tid = threadIdx.x;
   t.slot = tid >> s.log_tpi;
   t.tin = tid & (s.tpi - 1);
   t.lane = t.tin & (s.lanes - 1);
   t.row = t.tin >> s.log_lanes;
-  t.b = (int)ib * s.nb + t.slot;
-  t.v = t.chunk * s.cv + t.lane;
-  t.live = t.slot < s.nb && t.b < g.B && t.lane < s.cv && t.v < g.nv;
-  t.b = min(t.b, g.B - 1);
-  t.v = min(t.v, g.nv - 1);
+  t.v = min(t.chunk * s.cv + t.lane, g.nv - 1);
+  slab_item(g, s, item, t);
   return t;
 }
 // The pixels of a part: first, how many there are, how many of them are this thread's.
@@ -781,17 +783,6 @@ __global__ __launch_bounds__(kThreads) void gn_bwd_apply_kernel(const NormArgs a
     if (w.live && i < w.n) store_stream(out + (int64_t)p * a.ocs, ActVec<T>::pack(dx));
   }
 }
-// h, and z where the activation's slope needs it, of channels e0 .. e0 + 3 of a vector.
-template <int NS, int N, int ACT>
-__device__ __forceinline__ void norm_z(int e0, const float* x, const float* mean, const float* rstd, const float* gamma, const float* beta,
-                                       float* h, float* z) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int k = (e0 + j) * NS / N;
-    h[j] = (x[j] - mean[k]) * rstd[k];
-    if (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) z[j] = fmaf(h[j], gamma[e0 + j], beta[e0 + j]);
-  }
-}
 // ReLU's gate is a border that fp32 rounding of z may cross.  But z > 0 is  sign(gamma) x > sign(gamma) tau  with
 // tau = mean - beta / (rstd gamma), and x is an fp32 value: against tau in 64 bits, rounded down to fp32, the comparison is
 // exact.  A channel's tau is worked out once per workgroup; the gate costs two instructions and needs no z.
@@ -825,16 +816,24 @@ __device__ __forceinline__ void relu_thresholds(const NormArgs& a, const Slab& s
   for (int j = 0; j < N; ++j) out[j] = mine[t.lane * N + j];
   __syncthreads();
 }
-template <int NS, int N>
-__device__ __forceinline__ void slab_channels(const NormArgs& a, int b, int c0, float* mean, float* rstd, float* gamma, float* beta) {
+template <int NS, int N> __device__ __forceinline__ void slab_stats(const NormArgs& a, int b, int c0, float* mean, float* rstd) {
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
     const int64_t gi = (int64_t)b * a.g.G + fdiv((uint32_t)min(c0 + j * N / NS, a.g.C - 1), a.g.d_cg);
     mean[j] = a.mean[gi];
     rstd[j] = a.rstd[gi];
   }
-  load_channels<N>(a.gamma, 1.f, c0, a.g.C, gamma);
+}
+// Per-channel values of the backward pass: scaled = gamma * rstd.
+template <int NS, int N>
+__device__ __forceinline__ void slab_channels(const NormArgs& a, int b, int c0, float* mean, float* rstd, float* scaled, float* beta) {
+  slab_stats<NS, N>(a, b, c0, mean, rstd);
+  load_channels<N>(a.gamma, 1.f, c0, a.g.C, scaled);
   load_channels<N>(a.beta, 0.f, c0, a.g.C, beta);
+}
+template <int NS, int N> __device__ __forceinline__ void slab_scale(const float* rstd, float* scaled) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) scaled[j] *= rstd[j * NS / N];
 }
 __device__ __forceinline__ int opaque(int v) {                   // a value whose uses are not prepared in advance
   asm volatile("" : "+v"(v));
@@ -882,45 +881,47 @@ __device__ __forceinline__ void store_channel(const NormArgs& a, int row, int c,
   if (a.dgamma) a.dgamma[c] = a.ga * sum_dzh + (a.gb != 0.f ? a.gb * a.dgamma[c] : 0.f);
   if (a.dbeta) a.dbeta[c] = a.ga * sum_dz + (a.gb != 0.f ? a.gb * a.dbeta[c] : 0.f);
 }
-// Adds a vector's dz and dz * h to the sums of its channels (d4: dy, dropped units cleared).  What the second pass needs of
-// dy comes back: with gated-off units cleared, in fp32 as dz itself (a bf16 dz would be rounded: its slope is worked out again).
+// Adds a vector's dz and dz * (x - mean) to the sums of its channels (d4: dy, dropped units cleared; scaled: gamma * rstd).
+// What the second pass needs of dy comes back: with gated-off units cleared, in fp32 as dz itself (a bf16 dz would be
+// rounded: its slope is worked out again).
 template <typename T, int NS, int ACT>
-__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const float* mean, const float* rstd, const float* gamma,
-                                         const float* beta, const float* threshold, float* ch) {
+__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const float* mean, const float* scaled, const float* beta,
+                                         const float* threshold, float* ch) {
   constexpr int N = ActVec<T>::N;
 #pragma unroll
   for (int e = 0; e < N / 4; ++e) {
-    float x[4], d[4], h[4], z[4];
+    float x[4], d[4];
     ActVec<T>::unpack4(x4, e, x);
     ActVec<T>::unpack4(d4, e, d);
-    norm_z<NS, N, ACT>(4 * e, x, mean, rstd, gamma, beta, h, z);
     if constexpr (ACT == MI_ACT_RELU) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] = relu_gate(x[j], gamma[4 * e + j], threshold[4 * e + j]) ? d[j] : 0.f;
+      for (int j = 0; j < 4; ++j) d[j] = relu_gate(x[j], scaled[4 * e + j], threshold[4 * e + j]) ? d[j] : 0.f;
       ActVec<T>::pack4_exact(d, e, d4);
-      if (e == N / 4 - 1) pin(d4, rstd[0]);                      // what was packed is not kept unpacked besides
+      if (e == N / 4 - 1) pin(d4, mean[0]);                      // what was packed is not kept unpacked besides
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] -= mean[(4 * e + j) * NS / N];
     if constexpr (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(z[j]);
+      for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[4 * e + j], beta[4 * e + j]));
     }
     if constexpr (N == 4 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) ActVec<T>::pack4(d, e, d4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       ch[4 * e + j] += d[j];
-      ch[N + 4 * e + j] = fmaf(d[j], h[j], ch[N + 4 * e + j]);
+      ch[N + 4 * e + j] = fmaf(d[j], x[j], ch[N + 4 * e + j]);
     }
     __builtin_amdgcn_sched_barrier(0);                           // one group after the other: together they need several times the registers
   }
 }
-// A group's two sums from those of a thread's channels.
-template <int NS, int N> __device__ __forceinline__ void bwd_group_sums(const float* ch, const float* gamma, float (&sum)[2][NS]) {
+// A group's two sums, of rstd * t and rstd * t * (x - mean), from those of a thread's channels.
+template <int NS, int N> __device__ __forceinline__ void bwd_group_sums(const float* ch, const float* scaled, float (&sum)[2][NS]) {
 #pragma unroll
   for (int j = 0; j < NS; ++j) sum[0][j] = sum[1][j] = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    sum[0][j * NS / N] = fmaf(gamma[j], ch[j], sum[0][j * NS / N]);
-    sum[1][j * NS / N] = fmaf(gamma[j], ch[N + j], sum[1][j * NS / N]);
+    sum[0][j * NS / N] = fmaf(scaled[j], ch[j], sum[0][j * NS / N]);
+    sum[1][j * NS / N] = fmaf(scaled[j], ch[N + j], sum[1][j * NS / N]);
   }
 }
 // The sums of a part whose workgroup has not come, from memory: the same operations in the same order, one vector at a time.
@@ -930,8 +931,9 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
   const NormGeom& g = a.g;
   const SlabPixels px = slab_pixels<I>(t, g, s, part);
   const int c0 = opaque(t.v * N), chunk_c0 = t.chunk * s.cv * N;
-  float mean[NS], rstd[NS], gamma[N], beta[N], threshold[N], ch[2 * N] = {}, sum[2][NS];
-  slab_channels<NS, N>(a, t.b, c0, mean, rstd, gamma, beta);
+  float mean[NS], rstd[NS], scaled[N], beta[N], threshold[N], ch[2 * N] = {}, sum[2][NS];
+  slab_channels<NS, N>(a, t.b, c0, mean, rstd, scaled, beta);
+  slab_scale<NS, N>(rstd, scaled);
   if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, relu_inputs(a, t, chunk_c0, t.tin), shared, threshold);
   const auto x = in_memory<T, I>(t, px, g, s, a.x, a.xcs, a.xco), dy = in_memory<T, I>(t, px, g, s, a.dy, a.ycs, a.yco);
 #pragma unroll 1
@@ -943,80 +945,58 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
       keep.add(0, a.drop, drop_offset(a.drop), row * (uint32_t)(g.nv * N) + c0);
       d = keep.kept(0, d);
     }
-    bwd_step<T, NS, ACT>(x(i, 0.f), d, mean, rstd, gamma, beta, threshold, ch);
+    bwd_step<T, NS, ACT>(x(i, 0.f), d, mean, scaled, beta, threshold, ch);
   }
-  bwd_group_sums<NS, N>(ch, gamma, sum);
+  bwd_group_sums<NS, N>(ch, scaled, sum);
   slab_sum<NS, 2>(sum, g, s, t, shared);
   publish_bwd<NS, N>(a, t, part, sum);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the next look finds it
 }
-// One read of x and dy: the same division of the work as forward.  Sums of dz and dz * h for each channel come first; a
-// group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
-// linear in it.
-template <typename T, int NS, int I, bool PARTS, int ACT>
-__global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
-  constexpr int N = ActVec<T>::N, Q = N / NS;
-  extern __shared__ float shared[];
-  const NormGeom& g = a.g;
-  const SlabThread t = slab_thread(g, s);
-  const int c0 = t.v * N, chunk_c0 = t.chunk * s.cv * N;
-  const float scale = a.drop.on ? a.drop.scale : 1.f;
-  const SlabPixels px = slab_pixels<I>(t, g, s, t.part);
-  u32x4_t vx[I], vd[I];
-  float mean[NS], rstd[NS], gamma[N], beta[N], threshold[N];
-  float sum[2][NS];                                              // then the means of t and t * h
-  {
-    ReluInputs first;
-    if constexpr (ACT == MI_ACT_RELU) first = relu_inputs(a, t, chunk_c0, t.tin);
-    slab_channels<NS, N>(a, t.b, c0, mean, rstd, gamma, beta);
-    load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, vx);
-    load_slab<T, I>(t, px, g, s, a.dy, a.ycs, a.yco, vd);
-    if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, first, shared, threshold);
-    if (a.drop.on) {
-      KeepBits<I, N> keep;                                       // while the loads are in flight
-      const uint64_t offset = drop_offset(a.drop);
+// The mask of a part's units, applied to dy's registers.
+template <typename T, int I>
+__device__ __forceinline__ void bwd_drop(const NormArgs& a, const Slab& s, const SlabThread& t, const SlabPixels& px, u32x4_t (&vd)[I]) {
+  constexpr int N = ActVec<T>::N;
+  if (!a.drop.on) return;
+  KeepBits<I, N> keep;
+  const uint64_t offset = drop_offset(a.drop);
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const uint64_t row = a.drop.per_channel ? (uint64_t)t.b : (uint64_t)t.b * g.P + (px.first + t.row + i * s.rows);
-        keep.add(i, a.drop, offset, row * (uint32_t)(g.nv * N) + c0);
-      }
-#pragma unroll
-      for (int i = 0; i < I; ++i) vd[i] = keep.kept(i, vd[i]);
-    }
-    zero_missing(px, vx);
-    zero_missing(px, vd);
-    float ch[2 * N] = {};                                        // sum dz, sum dz * h of each channel
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-      pin(vx[i], rstd[0]);
-      pin(vd[i], rstd[0]);
-      bwd_step<T, NS, ACT>(vx[i], vd[i], mean, rstd, gamma, beta, threshold, ch);
-    }
-    bwd_group_sums<NS, N>(ch, gamma, sum);
-    slab_sum<NS, 2>(sum, g, s, t, shared);
-    if constexpr (PARTS) publish_bwd<NS, N>(a, t, t.part, sum);
-    if (a.dgamma != nullptr || a.dbeta != nullptr) {
-      // the workgroup's sums of each channel, over rows and images: lanes first, each stage halves what a lane holds
-      __syncthreads();
-      const int lane = threadIdx.x & 63, waves = s.threads >> 6;
-      if (!t.live) {
-#pragma unroll
-        for (int j = 0; j < 2 * N; ++j) ch[j] = 0.f;
-      }
-      scatter_sum<2 * N>(ch, 32, s.lanes, lane, shared + ((threadIdx.x >> 6) * s.lanes + (lane & (s.lanes - 1))) * (2 * N));
-      __syncthreads();
-      for (int k = threadIdx.x; k < s.lanes * N; k += s.threads) {
-        const int l = k / N, j = k & (N - 1), c = chunk_c0 + k;
-        if (l >= s.cv || c >= g.C) continue;
-        float sa = 0.f, sq = 0.f;
-        for (int w = 0; w < waves; ++w) {
-          sa += shared[(w * s.lanes + l) * 2 * N + j];
-          sq += shared[(w * s.lanes + l) * 2 * N + N + j];
-        }
-        store_channel(a, (int)(blockIdx.x / s.chunks), c, sa * scale, sq * scale);
-      }
-    }
+  for (int i = 0; i < I; ++i) {
+    const uint64_t row = a.drop.per_channel ? (uint64_t)t.b : (uint64_t)t.b * a.g.P + (px.first + t.row + i * s.rows);
+    keep.add(i, a.drop, offset, row * (uint32_t)(a.g.nv * N) + t.v * N);
   }
+#pragma unroll
+  for (int i = 0; i < I; ++i) vd[i] = keep.kept(i, vd[i]);
+}
+// The workgroup's sums of each channel, over rows and images, into row `row` of the parameter gradients: lanes first, each
+// stage halves what a lane holds, then the waves through LDS.
+template <int N>
+__device__ __forceinline__ void bwd_channel_sums(const NormArgs& a, const Slab& s, const SlabThread& t, float (&ch)[2 * N], bool live,
+                                                 float scale, int row, float* shared) {
+  if (a.dgamma == nullptr && a.dbeta == nullptr) return;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, waves = s.threads >> 6, c0 = t.chunk * s.cv * N;
+  if (!live) {
+#pragma unroll
+    for (int j = 0; j < 2 * N; ++j) ch[j] = 0.f;
+  }
+  scatter_sum<2 * N>(ch, 32, s.lanes, lane, shared + ((threadIdx.x >> 6) * s.lanes + (lane & (s.lanes - 1))) * (2 * N));
+  __syncthreads();
+  for (int k = threadIdx.x; k < s.lanes * N; k += s.threads) {
+    const int l = k / N, j = k & (N - 1), c = c0 + k;
+    if (l >= s.cv || c >= a.g.C) continue;
+    float sa = 0.f, sq = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      sa += shared[(w * s.lanes + l) * 2 * N + j];
+      sq += shared[(w * s.lanes + l) * 2 * N + N + j];
+    }
+    store_channel(a, row, c, sa * scale, sq * scale);
+  }
+}
+// The means over the groups of a thread's pieces, from all parts of the image; `sum` has this part's sums.
+template <typename T, int NS, int I, bool PARTS, int ACT>
+__device__ __forceinline__ void bwd_means(const NormArgs& a, const Slab& s, const SlabThread& t, float (&sum)[2][NS], float* shared) {
+  constexpr int N = ActVec<T>::N;
+  const NormGeom& g = a.g;
   if constexpr (!PARTS) {
     const float inv = 1.f / ((float)g.P * (float)g.cg);
 #pragma unroll
@@ -1025,7 +1005,7 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kerne
       sum[1][j] *= inv;
     }
   } else {
-    const int g0 = chunk_c0 / g.cg, groups = min(s.cv * N / g.cg, g.G - g0);
+    const int g0 = t.chunk * s.cv * N / g.cg, groups = min(s.cv * N / g.cg, g.G - g0);
     const uint64_t* words = a.words + ((int64_t)t.b * s.parts * g.G + g0);
     float* stats = shared + slab_stats_at<NS>(s);
     __syncthreads();
@@ -1045,41 +1025,51 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kerne
     }
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int gi = (int)fdiv((uint32_t)min(c0 + j * Q, g.C - 1), g.d_cg) - g0;
+      const int gi = (int)fdiv((uint32_t)min(t.v * N + j * (N / NS), g.C - 1), g.d_cg) - g0;
       sum[0][j] = stats[2 * gi];
       sum[1][j] = stats[2 * gi + 1];
     }
-    slab_channels<NS, N>(a, t.b, opaque(c0), mean, rstd, gamma, beta);   // the exchange needs their registers
   }
-  T* out = (T*)a.out + ((int64_t)t.b * g.P + px.first + t.row) * a.ocs + a.oco + c0;
-  const bool tail = c0 + N > g.C;
-  float rscale[NS];
+}
+// dx of a part from the registers:  dx = scaled * dz - M1 - (x - mean) * rstd^2 * M2,  M1 and M2 the means over the group of
+// scaled * dz and scaled * dz * (x - mean); times dropout's factor.
+template <typename T, int NS, int I, int ACT>
+__device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const SlabThread& t, const SlabPixels& px, u32x4_t (&vx)[I],
+                                         u32x4_t (&vd)[I], const float* mean, const float* rstd, const float* scaled, const float* beta,
+                                         const float (&sum)[2][NS], float factor) {
+  constexpr int N = ActVec<T>::N, Q = N / NS;
+  const int c0 = t.v * N;
+  T* out = (T*)a.out + ((int64_t)t.b * a.g.P + px.first + t.row) * a.ocs + a.oco + c0;
+  const bool tail = c0 + N > a.g.C;
+  // a group of one value passes nothing on; its terms would cancel but for their roundings
+  if (a.g.P == 1 && a.g.cg == 1) factor = 0.f;
+  float b0[NS], b1[NS], slope[N];
 #pragma unroll
-  for (int j = 0; j < NS; ++j) rscale[j] = rstd[j] * scale;
+  for (int j = 0; j < NS; ++j) {
+    b0[j] = -sum[0][j] * factor;
+    b1[j] = -sum[1][j] * rstd[j] * rstd[j] * factor;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) slope[j] = scaled[j] * factor;
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     pin(vx[i], sum[0][0]);
     pin(vd[i], sum[0][0]);
 #pragma unroll
     for (int e = 0; e < N / 4; ++e) {
-      float x[4], d[4], h[4], z[4];
+      float x[4], d[4];
       ActVec<T>::unpack4(vx[i], e, x);
       ActVec<T>::unpack4(vd[i], e, d);
-      norm_z<NS, N, ACT>(4 * e, x, mean, rstd, gamma, beta, h, z);
-      if constexpr (N == 8 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(z[j]);
-      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-#pragma clang fp contract(off)   // t is rounded before the subtraction, as it was in the sum: a group of one value gives exactly zero
-        const int k = (4 * e + j) / Q;
-        const float tj = gamma[4 * e + j] * d[j];
-        d[j] = rscale[k] * fmaf(-h[j], sum[1][k], tj - sum[0][k]);
+        const int c = 4 * e + j, k = c / Q;
+        x[j] -= mean[k];
+        if constexpr (N == 8 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[c], beta[c]));
+        d[j] = fmaf(x[j], b1[k], fmaf(d[j], slope[c], b0[k]));
       }
       if (tail) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] = c0 + 4 * e + j < g.C ? d[j] : 0.f;
+        for (int j = 0; j < 4; ++j) d[j] = c0 + 4 * e + j < a.g.C ? d[j] : 0.f;
       }
       ActVec<T>::pack4(d, e, vd[i]);
       __builtin_amdgcn_sched_barrier(0);
@@ -1087,7 +1077,49 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kerne
     if (t.live && i < px.mine) store_stream(out + (int64_t)(i * s.rows) * a.ocs, vd[i]);
   }
 }
-
+// One read of x and dy: the same division of the work as forward.  Sums of dz and dz * h for each channel come first; a
+// group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
+// linear in it.
+template <typename T, int NS, int I, bool PARTS, int ACT>
+__global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
+  constexpr int N = ActVec<T>::N;
+  extern __shared__ float shared[];
+  const NormGeom& g = a.g;
+  const SlabThread t = slab_thread(g, s);
+  const int c0 = t.v * N;
+  const float scale = a.drop.on ? a.drop.scale : 1.f;
+  const SlabPixels px = slab_pixels<I>(t, g, s, t.part);
+  u32x4_t vx[I], vd[I];
+  float mean[NS], rstd[NS], scaled[N], beta[N], threshold[N], sum[2][NS], ch[2 * N] = {};
+  ReluInputs first;
+  if constexpr (ACT == MI_ACT_RELU) first = relu_inputs(a, t, t.chunk * s.cv * N, t.tin);
+  slab_channels<NS, N>(a, t.b, c0, mean, rstd, scaled, beta);
+  load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, vx);
+  load_slab<T, I>(t, px, g, s, a.dy, a.ycs, a.yco, vd);
+  if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, first, shared, threshold);
+  slab_scale<NS, N>(rstd, scaled);
+  bwd_drop<T, I>(a, s, t, px, vd);
+  zero_missing(px, vx);
+  zero_missing(px, vd);
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    pin(vx[i], scaled[0]);
+    pin(vd[i], scaled[0]);
+    bwd_step<T, NS, ACT>(vx[i], vd[i], mean, scaled, beta, threshold, ch);
+  }
+  bwd_group_sums<NS, N>(ch, scaled, sum);
+  slab_sum<NS, 2>(sum, g, s, t, shared);
+  if constexpr (PARTS) publish_bwd<NS, N>(a, t, t.part, sum);
+#pragma unroll
+  for (int j = 0; j < N; ++j) ch[N + j] *= rstd[j * NS / N];     // dz * h
+  bwd_channel_sums<N>(a, s, t, ch, t.live, scale, (int)(blockIdx.x / s.chunks), shared);
+  bwd_means<T, NS, I, PARTS, ACT>(a, s, t, sum, shared);
+  if constexpr (PARTS) {                                         // the exchange needs their registers
+    slab_channels<NS, N>(a, t.b, opaque(c0), mean, rstd, scaled, beta);
+    slab_scale<NS, N>(rstd, scaled);
+  }
+  bwd_emit<T, NS, I, ACT>(a, s, t, px, vx, vd, mean, rstd, scaled, beta, sum, scale);
+}
 // ---------------------------------------------------------------- launches
 // in norm.hip
 void launch_gn_empty(uint64_t* words, int64_t n, hipStream_t s);
