@@ -198,18 +198,21 @@ int mi_dropout_fwd(const void* x, int x_cstride, int x_coff, const void* residua
 /* y = dropout(act((x - mean) * rstd * gamma + beta)): torch's nn.GroupNorm(groups, C, eps), an activation and a
  * dropout (drop may be NULL) in one operator.  gamma, beta: C floats each, or NULL (1 and 0).  mean, rstd
  * (B*groups floats each) are written; the backward pass reads them.  C must be a multiple of groups.  y must not
- * overlap x.  ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content (NULL where that is 0). */
+ * overlap x.  ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content (NULL where that is 0).
+ * Several workgroups may share a large image; each then looks for the others' sums, at most `polls` times, and forms
+ * those that have not come itself, so that no call depends on its workgroups running at the same time.  polls < 0: the
+ * library's choice (some milliseconds).  The result does not depend on it, bit for bit. */
 int mi_group_norm_act_fwd(const void* x, int x_cstride, int x_coff, const float* gamma, const float* beta,
                           void* y, int y_cstride, int y_coff, float* mean, float* rstd,
-                          int B, int H, int W, int C, int groups, int act, float eps, const mi_dropout* drop,
+                          int B, int H, int W, int C, int groups, int act, float eps, const mi_dropout* drop, int polls,
                           void* ws, size_t ws_bytes, int dtype, mi_stream s);
 /* dx, and dgamma = alpha*sum + beta_acc*dgamma, dbeta likewise (either may be NULL).  x, mean, rstd, gamma, beta, act
  * and drop as in the forward pass; ReLU has slope 0 at 0.  dx must not overlap x or dy.  Sums have a fixed order:
- * the same call gives the same bits.  ws: mi_group_norm_ws_bytes(..., 1, ...) bytes, any content. */
+ * the same call gives the same bits.  polls, ws (mi_group_norm_ws_bytes(..., 1, ...) bytes): as above. */
 int mi_group_norm_act_bwd(const void* x, int x_cstride, int x_coff, const void* dy, int dy_cstride, int dy_coff,
                           const float* gamma, const float* beta, const float* mean, const float* rstd,
                           void* dx, int dx_cstride, int dx_coff, float* dgamma, float* dbeta, float alpha, float beta_acc,
-                          int B, int H, int W, int C, int groups, int act, const mi_dropout* drop,
+                          int B, int H, int W, int C, int groups, int act, const mi_dropout* drop, int polls,
                           void* ws, size_t ws_bytes, int dtype, mi_stream s);
 size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backward, int dtype);
 

@@ -65,13 +65,13 @@ A = 1 << 20          # an aligned address that nothing may touch
 def _norm_fwd(L, x=A, xcs=64, xco=0, gamma=None, y=A << 4, ycs=64, yco=0, mean=A, rstd=A, B=2, H=4, W=4, Cc=40, G=5, act=1,
               eps=1e-5, drop=None, ws=A, ws_bytes=1 << 20, dt=0):
     return L.mi_group_norm_act_fwd(x, xcs, xco, gamma, None, y, ycs, yco, mean, rstd, B, H, W, Cc, G, act, eps,
-                                   C.byref(drop) if drop else None, ws, ws_bytes, dt, None)
+                                   C.byref(drop) if drop else None, -1, ws, ws_bytes, dt, None)
 
 
 def _norm_bwd(L, x=A, dy=A << 1, dx=A << 4, xcs=64, dcs=64, dco=0, mean=A, B=2, H=4, W=4, Cc=40, G=5, act=1, ws=A,
               ws_bytes=1 << 20, dt=1):
     return L.mi_group_norm_act_bwd(x, xcs, 0, dy, 64, 0, None, None, mean, A, dx, dcs, dco, None, None, 1.0, 0.0, B, H, W, Cc, G,
-                                   act, None, ws, ws_bytes, dt, None)
+                                   act, None, -1, ws, ws_bytes, dt, None)
 
 
 def _drop(L, x=A, xcs=64, xco=0, r=None, rcs=64, y=A << 4, ycs=64, yco=0, B=2, H=4, W=4, Cc=40, drop=None, dt=0):

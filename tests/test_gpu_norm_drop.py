@@ -268,6 +268,26 @@ def test_results_repeat(ua):
             assert all(torch.equal(s, t) for s, t in zip(runs[0], other))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ACTS)
+def test_sums_of_parts_that_have_not_come(ua, monkeypatch, dtype, kind):
+    """Images that several workgroups share, with no patience for each other: a workgroup that looks for the others' sums
+    once only forms the missing ones itself, and every bit is the same."""
+    ops = ua.ops
+    for B, H, W, C, G in ((3, 190, 150, 32, 8), (40, 80, 60, 48, 1), (2, 128, 128, 40, 5), (300, 33, 32, 32, 2), (1, 256, 256, 32, 32)):
+        x, dy = place(rnd(1, B, H, W, C, shift=3.0), dtype), place(rnd(2, B, H, W, C), dtype)
+        w, b = rnd(3, C).cuda(), rnd(4, C).cuda()
+        drop = ops.Drop(0.2, 9)
+        y, m, r = ops.group_norm_act_fwd(x, C, G, w, b, act=kind, drop=drop)
+        want = (y, m, r) + ops.group_norm_act_bwd(x, dy, m, r, C, G, w, b, act=kind, drop=drop)
+        monkeypatch.setattr(ops, "_POLLS", 0)
+        for _ in range(2):
+            y, m, r = ops.group_norm_act_fwd(x, C, G, w, b, act=kind, drop=drop)
+            got = (y, m, r) + ops.group_norm_act_bwd(x, dy, m, r, C, G, w, b, act=kind, drop=drop)
+            assert all(torch.equal(s, t) for s, t in zip(want, got)), (B, H, W, C, G)
+        monkeypatch.setattr(ops, "_POLLS", -1)
+
+
 def test_gradient_against_differences(ua):
     """<dL/dv, d> against (L(v + e d) - L(v - e d)) / 2 e for L = sum(dy * y), y from the kernel, v each input.
     The central difference is off by e^2 |L'''| / 6 (e = 2^-6, third derivatives of order 10 |d|^3 here: below 1e-3 of

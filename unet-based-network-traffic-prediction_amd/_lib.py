@@ -58,8 +58,8 @@ SIGNATURES = {
     "mi_conv1x1_head_bwd": (_i, _VIEW + [_p, _p] + _VIEW + [_p, _p, _f, _f, _p, _sz] + [_i] * 7 + [_p]),
     "mi_conv1x1_head_ws_bytes": (_sz, [_i, _i]),
     "mi_dropout_fwd": (_i, _VIEW + _VIEW + _VIEW + [_i] * 4 + [_p, _i, _p]),
-    "mi_group_norm_act_fwd": (_i, _VIEW + [_p, _p] + _VIEW + [_p, _p] + [_i] * 6 + [_f, _p, _p, _sz, _i, _p]),
-    "mi_group_norm_act_bwd": (_i, _VIEW + _VIEW + [_p] * 4 + _VIEW + [_p, _p, _f, _f] + [_i] * 6 + [_p, _p, _sz, _i, _p]),
+    "mi_group_norm_act_fwd": (_i, _VIEW + [_p, _p] + _VIEW + [_p, _p] + [_i] * 6 + [_f, _p, _i, _p, _sz, _i, _p]),
+    "mi_group_norm_act_bwd": (_i, _VIEW + _VIEW + [_p] * 4 + _VIEW + [_p, _p, _f, _f] + [_i] * 6 + [_p, _i, _p, _sz, _i, _p]),
     "mi_group_norm_ws_bytes": (_sz, [_i] * 7),
     "mi_mse_fwd_bwd": (_i, [_p, _p, _i64, _p, _p, _f, _p, _p, _sz, _p]),
     "mi_mse_ws_bytes": (_sz, [_i64]),

@@ -598,19 +598,19 @@ size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backwa
   MI_REQUIRE(B == 0 || ((ws != nullptr || ws_bytes == 0) && ((uintptr_t)ws & 15) == 0), what ": workspace missing or unaligned")
 int mi_group_norm_act_fwd(const void* x, int xcs, int xco, const float* gamma, const float* beta, void* y, int ycs, int yco,
                           float* mean, float* rstd, int B, int H, int W, int C, int groups, int act, float eps,
-                          const mi_dropout* drop, void* ws, size_t ws_bytes, int dtype, mi_stream s) {
+                          const mi_dropout* drop, int polls, void* ws, size_t ws_bytes, int dtype, mi_stream s) {
   MI_NORM_ARGS("group_norm_act_fwd");
   MI_REQUIRE(eps >= 0.f, "group_norm_act_fwd: eps must not be negative");
   MI_REQUIRE(B == 0 || (view_ok(x, xcs, xco, C) && view_ok(y, ycs, yco, C)),
              "group_norm_act_fwd: bad view (null, unaligned, or channels outside the stride)");
   MI_REQUIRE(!views_overlap(x, xcs, xco, y, ycs, yco, (int64_t)B * H * W, C, dtype), "group_norm_act_fwd: y overlaps x");
-  return launch_group_norm_fwd(x, xcs, xco, gamma, beta, y, ycs, yco, mean, rstd, B, H, W, C, groups, act, eps, drop, ws,
-                               ws_bytes, dtype, (hipStream_t)s);
+  return launch_group_norm_fwd(x, xcs, xco, gamma, beta, y, ycs, yco, mean, rstd, B, H, W, C, groups, act, eps, drop, polls,
+                               ws, ws_bytes, dtype, (hipStream_t)s);
 }
 int mi_group_norm_act_bwd(const void* x, int xcs, int xco, const void* dy, int ycs, int yco, const float* gamma, const float* beta,
                           const float* mean, const float* rstd, void* dx, int dcs, int dco, float* dgamma, float* dbeta,
                           float alpha, float beta_acc, int B, int H, int W, int C, int groups, int act, const mi_dropout* drop,
-                          void* ws, size_t ws_bytes, int dtype, mi_stream s) {
+                          int polls, void* ws, size_t ws_bytes, int dtype, mi_stream s) {
   MI_NORM_ARGS("group_norm_act_bwd");
   MI_REQUIRE(B == 0 || (view_ok(x, xcs, xco, C) && view_ok(dy, ycs, yco, C) && view_ok(dx, dcs, dco, C)),
              "group_norm_act_bwd: bad view (null, unaligned, or channels outside the stride)");
@@ -618,7 +618,7 @@ int mi_group_norm_act_bwd(const void* x, int xcs, int xco, const void* dy, int y
   MI_REQUIRE(!views_overlap(x, xcs, xco, dx, dcs, dco, px, C, dtype) && !views_overlap(dy, ycs, yco, dx, dcs, dco, px, C, dtype),
              "group_norm_act_bwd: dx overlaps x or dy");
   return launch_group_norm_bwd(x, xcs, xco, dy, ycs, yco, gamma, beta, mean, rstd, dx, dcs, dco, dgamma, dbeta, alpha, beta_acc,
-                               B, H, W, C, groups, act, drop, ws, ws_bytes, dtype, (hipStream_t)s);
+                               B, H, W, C, groups, act, drop, polls, ws, ws_bytes, dtype, (hipStream_t)s);
 }
 
 int mi_convt2x2_fwd(const void* x, int xcs, int xco, const void* wfwd, const float* bias, void* y, int ycs, int yco,

@@ -228,11 +228,11 @@ int launch_dropout(const void* x, int xcs, int xco, const void* r, int rcs, int 
 size_t group_norm_ws_bytes(int B, int H, int W, int C, int G, int backward, int dtype);
 int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, const float* beta, void* y, int ycs, int yco,
                           float* mean, float* rstd, int B, int H, int W, int C, int G, int act, float eps,
-                          const mi_dropout* drop, void* ws, size_t ws_bytes, int dtype, hipStream_t s);
+                          const mi_dropout* drop, int polls, void* ws, size_t ws_bytes, int dtype, hipStream_t s);
 int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int ycs, int yco, const float* gamma, const float* beta,
                           const float* mean, const float* rstd, void* dx, int dcs, int dco, float* dgamma, float* dbeta,
-                          float ga, float gb, int B, int H, int W, int C, int G, int act, const mi_dropout* drop, void* ws,
-                          size_t ws_bytes, int dtype, hipStream_t s);
+                          float ga, float gb, int B, int H, int W, int C, int G, int act, const mi_dropout* drop, int polls,
+                          void* ws, size_t ws_bytes, int dtype, hipStream_t s);
 int launch_mse(const float* pred, const float* target, int64_t n, float* out3, float* dpred, float gscale,
                const float* gscale_dev, void* ws, size_t ws_bytes, hipStream_t s);
 size_t mse_ws_bytes(int64_t n);

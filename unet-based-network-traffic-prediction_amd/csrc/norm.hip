@@ -135,7 +135,7 @@ static int pow2_ceil(int64_t v) {
 }
 // How the slab kernels divide the work, or false where they do not apply.
 constexpr int kMaxParts = 64;                // lanes of the wave that joins them
-constexpr int kPolls = 4096;
+constexpr int kPolls = 4096;                 // about 1 us each
 // The division with `iters` vectors a thread of chunks of cv vectors.
 static bool divide_slab(const NormGeom& g, int64_t cv, int iters, Slab* out) {
   Slab s{};
@@ -194,7 +194,7 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   if (vectors <= pow2_ceil(cv)) iters = 1;
   else if (alone) iters = pow2_ceil(g.B) * vectors <= few ? 4 : 16;
   else if (vectors > few && vectors <= most) iters = 16;
-  if (!divide_slab(g, cv, iters, out)) return false;
+  if (!divide_slab(g, cv, iters, out) && !divide_slab(g, cv, 16, out)) return false;
   out->by_xcd = out->chunks > 1 && out->cv < 8 && out->parts == 1 && out->img_blocks >= 8;
   return true;
 }
@@ -222,7 +222,7 @@ static int check_range(const NormGeom& g, const char* what) {
 }
 int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, const float* beta, void* y, int ycs, int yco,
                           float* mean, float* rstd, int B, int H, int W, int C, int G, int act, float eps,
-                          const mi_dropout* drop, void* ws, size_t ws_bytes, int dtype, hipStream_t s) {
+                          const mi_dropout* drop, int polls, void* ws, size_t ws_bytes, int dtype, hipStream_t s) {
   NormArgs a{};
   int rc = make_drop_args(drop, &a.drop);
   if (rc) return rc;
@@ -231,6 +231,7 @@ int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, c
   if (B == 0) return MI_OK;
   Slab slab;
   const Slab* sl = choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, false, &slab) ? &slab : nullptr;
+  if (polls >= 0) slab.polls = polls;
   if (ws_bytes < group_norm_ws_bytes(B, H, W, C, G, 0, dtype)) return fail(MI_ESIZE, "group_norm_act_fwd: workspace too small");
   a.x = x; a.xcs = xcs; a.xco = xco;
   a.out = y; a.ocs = ycs; a.oco = yco;
@@ -242,8 +243,8 @@ int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, c
 }
 int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int ycs, int yco, const float* gamma, const float* beta,
                           const float* mean, const float* rstd, void* dx, int dcs, int dco, float* dgamma, float* dbeta,
-                          float ga, float gb, int B, int H, int W, int C, int G, int act, const mi_dropout* drop, void* ws,
-                          size_t ws_bytes, int dtype, hipStream_t s) {
+                          float ga, float gb, int B, int H, int W, int C, int G, int act, const mi_dropout* drop, int polls,
+                          void* ws, size_t ws_bytes, int dtype, hipStream_t s) {
   NormArgs a{};
   int rc = make_drop_args(drop, &a.drop);
   if (rc) return rc;
@@ -257,6 +258,7 @@ int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int y
   a.act = act;
   Slab slab;
   const Slab* sl = B > 0 && choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, true, &slab) ? &slab : nullptr;
+  if (polls >= 0) slab.polls = polls;
   a.chan_stride = C;
   if (sl) {
     a.words = (uint64_t*)ws;

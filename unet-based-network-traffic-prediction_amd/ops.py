@@ -305,6 +305,7 @@ def _new_activation(x: torch.Tensor, C: int) -> torch.Tensor:
 # The small calls of these layers are bound by the host: ``torch.cuda.current_stream`` builds an object (1.8 us), this
 # returns the handle alone (0.1 us).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_POLLS = -1                  # see mi_group_norm_act_fwd
 
 
 def dropout_fwd(x, C, drop: Optional[Drop], residual=None, x_coff=0, residual_coff=0, out=None, out_coff=0):
@@ -353,7 +354,7 @@ def group_norm_act_fwd(x, C, groups, weight=None, bias=None, act="none", eps=1e-
         nbytes = _norm_ws_bytes(B, H, W, C, groups, 0, dt)
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
         check(lib().mi_group_norm_act_fwd(x.data_ptr(), cs, x_coff, wp, bp, out.data_ptr(), out.shape[3], out_coff, mean.data_ptr(),
-                                          rstd.data_ptr(), B, H, W, C, groups, code, eps, _drop_ref(drop, dev),
+                                          rstd.data_ptr(), B, H, W, C, groups, code, eps, _drop_ref(drop, dev), _POLLS,
                                           ws.data_ptr() if nbytes else None, nbytes, dt, _raw_stream(dev.index)), "group_norm_act_fwd")
     return out, mean, rstd
 
@@ -382,7 +383,7 @@ def group_norm_act_bwd(x, dy, mean, rstd, C, groups, weight=None, bias=None, act
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
         check(lib().mi_group_norm_act_bwd(x.data_ptr(), cs, x_coff, dy.data_ptr(), dy.shape[3], dy_coff, wp, bp, mp, rp,
                                           dx.data_ptr(), dx.shape[3], 0, gp, hp, alpha, beta, B, H, W, C, groups, code,
-                                          _drop_ref(drop, dev), ws.data_ptr() if nbytes else None, nbytes, dt,
+                                          _drop_ref(drop, dev), _POLLS, ws.data_ptr() if nbytes else None, nbytes, dt,
                                           _raw_stream(dev.index)), "group_norm_act_bwd")
     return dx, dweight, dbias
 
