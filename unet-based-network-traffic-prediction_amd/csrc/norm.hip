@@ -194,9 +194,7 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   if (vectors <= pow2_ceil(cv)) iters = 1;
   else if (alone) iters = pow2_ceil(g.B) * vectors <= few ? 4 : 16;
   else if (vectors > few && vectors <= most) iters = 16;
-  if (!divide_slab(g, cv, iters, out) && !divide_slab(g, cv, 16, out)) return false;
-  out->by_xcd = out->chunks > 1 && out->cv < 8 && out->parts == 1 && out->img_blocks >= 8;
-  return true;
+  return divide_slab(g, cv, iters, out) || divide_slab(g, cv, 16, out);
 }
 static size_t slab_rows(const Slab& s) { return (size_t)s.img_blocks * s.parts; }   // rows of channel sums
 static size_t fwd_part_bytes(const NormGeom& g) { return (size_t)g.B * g.tiles * g.nv * g.n_slots * sizeof(float4); }

@@ -287,7 +287,6 @@ struct Slab {
   int merge;                   // lanes of a group that shuffles can sum (a power of two), ...
   int left;                    // ... and what then remains: pieces per group / merge
   int threads, iters;          // nb * tpi, pixels per thread
-  int by_xcd;                  // chunks of an image go to one XCD: they share the lines that its L2 holds
   int polls;                   // how often a part is looked for before its sums are formed here instead
   FastDiv d_chunks, d_parts;
 };
@@ -306,15 +305,8 @@ __device__ __forceinline__ void slab_item(const NormGeom& g, const Slab& s, uint
 }
 __device__ __forceinline__ SlabThread slab_thread(const NormGeom& g, const Slab& s) {
   SlabThread t;
-  uint32_t item;
-  if (s.by_xcd) {                                                // workgroup i runs on XCD i % 8
-    const uint32_t i = blockIdx.x, j = i >> 3, q = fdiv(j, s.d_chunks);
-    t.chunk = (int)(j - q * s.chunks);
-    item = q * 8 + (i & 7);
-  } else {
-    item = fdiv(blockIdx.x, s.d_chunks);
-    t.chunk = (int)(blockIdx.x - item * s.chunks);
-  }
+  const uint32_t item = fdiv(blockIdx.x, s.d_chunks);
+  t.chunk = (int)(blockIdx.x - item * s.chunks);
   const int tid = threadIdx.x;
   t.slot = tid >> s.log_tpi;
   t.tin = tid & (s.tpi - 1);
@@ -1127,9 +1119,7 @@ void launch_gn_join(const NormArgs& a, hipStream_t s);
 void launch_gn_bwd_join(const NormArgs& a, int padded, hipStream_t s);
 void launch_gn_param_grads(const NormArgs& a, hipStream_t s);
 
-inline unsigned slab_grid(const Slab& s) {
-  return (unsigned)((s.by_xcd ? (s.img_blocks + 7) / 8 * 8 : s.img_blocks * s.parts) * s.chunks);
-}
+inline unsigned slab_grid(const Slab& s) { return (unsigned)(s.img_blocks * s.parts * s.chunks); }
 // 64-bit words that the parts exchange
 inline int64_t slab_words(const NormGeom& g, const Slab& s) { return 2 * (int64_t)g.B * s.parts * g.G; }
 // LDS floats of slab_sum with K sums of NS pieces
