@@ -639,7 +639,7 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_fwd_slab_kerne
 #pragma unroll
   for (int j = 0; j < N; ++j) gamma[j] *= rstd[j / Q];           // z = (x - mean) * (rstd * gamma) + beta
   T* out = (T*)a.out + ((int64_t)t.b * g.P + px.first + t.row) * a.ocs + a.oco + c0;
-  const bool tail = c0 + N > g.C;
+  const bool ragged = g.C != g.nv * N;                           // uniform: mostly there are no padding channels to look for
   auto emit = [&](auto act) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
@@ -652,7 +652,7 @@ __global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_fwd_slab_kerne
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = keep.kept(i, j, f[j] * a.drop.scale);
       }
-      if (tail) {
+      if (ragged) {
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = c0 + j < g.C ? f[j] : 0.f;
       }
@@ -1032,7 +1032,7 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
   constexpr int N = ActVec<T>::N, Q = N / NS;
   const int c0 = t.v * N;
   T* out = (T*)a.out + ((int64_t)t.b * a.g.P + px.first + t.row) * a.ocs + a.oco + c0;
-  const bool tail = c0 + N > a.g.C;
+  const bool ragged = a.g.C != a.g.nv * N;
   // a group of one value passes nothing on; its terms would cancel but for their roundings
   if (a.g.P == 1 && a.g.cg == 1) factor = 0.f;
   float b0[NS], b1[NS], slope[N];
@@ -1059,7 +1059,7 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
         if constexpr (N == 8 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[c], beta[c]));
         d[j] = fmaf(x[j], b1[k], fmaf(d[j], slope[c], b0[k]));
       }
-      if (tail) {
+      if (ragged) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) d[j] = c0 + 4 * e + j < a.g.C ? d[j] : 0.f;
       }
