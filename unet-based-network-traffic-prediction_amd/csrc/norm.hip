@@ -68,10 +68,15 @@ __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const NormArgs a) 
   const int k = threadIdx.x & 7, r = threadIdx.x >> 3, c = blockIdx.x * 8 + k;
   float2 s = make_float2(0.f, 0.f);
   if (c < a.g.C) {
-    for (int row = r; row < a.chan_rows; row += 128) {
-      const float2 p = a.chan[(int64_t)row * a.chan_stride + c];
-      s.x += p.x;
-      s.y += p.y;
+    for (int row = r; row < a.chan_rows; row += 128 * 8) {       // eight loads in flight: the kernel is one memory latency long
+      float2 p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = a.chan[(int64_t)min(row + i * 128, a.chan_rows - 1) * a.chan_stride + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s.x += row + i * 128 < a.chan_rows ? p[i].x : 0.f;
+        s.y += row + i * 128 < a.chan_rows ? p[i].y : 0.f;
+      }
     }
   }
 #pragma unroll
