@@ -109,6 +109,7 @@ SHAPES = [  # B, H, W, C, groups
     (2, 16, 16, 64, 1), (2, 8, 8, 64, 64), (4, 4, 4, 512, 8), (2, 2, 2, 1024, 32), (1, 3, 5, 1040, 2), (1, 12, 11, 33, 3),
     (2, 70, 67, 36, 9), (5, 5, 5, 100, 25), (130, 2, 2, 48, 3), (1, 128, 128, 32, 8), (1, 7, 1, 528, 1), (2, 6, 6, 2080, 13),
     (1, 200, 210, 24, 2), (17, 16, 16, 128, 32), (18, 64, 64, 64, 32), (9, 64, 60, 48, 6), (33, 20, 20, 96, 12),
+    (257, 7, 7, 512, 8), (8, 4, 4, 1024, 32), (7, 23, 23, 96, 8), (3, 64, 64, 64, 8), (5, 16, 16, 64, 8), (40, 7, 5, 56, 56),
 ]
 
 

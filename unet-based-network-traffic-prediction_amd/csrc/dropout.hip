@@ -103,7 +103,7 @@ int launch_dropout(const void* x, int xcs, int xco, const void* r, int rcs, int 
   a.d_nv = make_fastdiv(a.nv);
   a.d_px = make_fastdiv(H * W);
   const int64_t blocks = (a.total + 256 * kU - 1) / (256 * kU);
-  MI_REQUIRE(blocks < (1ll << 31), "dropout: tensor too large");
+  MI_REQUIRE(blocks < (1ll << 24), "dropout: tensor too large");           // a launch holds less than 2^32 threads
   const dim3 grid((unsigned)blocks), block(256);
   if (dtype == MI_BF16) {
     if (r) hipLaunchKernelGGL((dropout_kernel<__bf16, true>), grid, block, 0, s, a);

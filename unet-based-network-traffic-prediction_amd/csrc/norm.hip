@@ -2,6 +2,8 @@
 // (norm_f32.hip, norm_bf16.hip; the kernels themselves are in norm_impl.h).
 #include "norm_impl.h"
 
+#include <algorithm>
+
 namespace mi {
 
 int launch_gn_fwd_f32(const NormArgs& a, const Slab* sl, hipStream_t s);
@@ -139,10 +141,12 @@ static int pow2_ceil(int64_t v) {
   return p;
 }
 // How the slab kernels divide the work, or false where they do not apply.
-constexpr int kMaxParts = 64;                // lanes of the wave that joins them
+// Up to 64 parts: the lanes of the wave that joins them.  Without parts, by the general kernels: 16 images of 128x128x64
+// bf16 20 us forward and 75 backward, with them 14 and 25; 2 of 256x256x32 12.7 and 50 against 13.6 and 20.
+constexpr int kMaxParts = 64;
 constexpr int kPolls = 4096;                 // about 1 us each
-// The division with `iters` vectors a thread of chunks of cv vectors.
-static bool divide_slab(const NormGeom& g, int64_t cv, int iters, Slab* out) {
+// The division with `iters` vectors a thread of chunks of cv vectors, up to `most` threads for an image, `most_nb` for several.
+static bool divide_slab(const NormGeom& g, int64_t cv, int iters, int most, int most_nb, Slab* out) {
   Slab s{};
   s.iters = iters;
   s.cv = (int)cv;
@@ -150,7 +154,7 @@ static bool divide_slab(const NormGeom& g, int64_t cv, int iters, Slab* out) {
   while ((1 << s.log_lanes) < s.lanes) ++s.log_lanes;
   s.chunks = (int)((g.nv + cv - 1) / cv);
   const int64_t vectors = (int64_t)g.P * s.lanes;
-  s.tpi = vectors < iters * kSlabThreads ? pow2_ceil((vectors + iters - 1) / iters) : kSlabThreads;
+  s.tpi = vectors < iters * most ? pow2_ceil((vectors + iters - 1) / iters) : most;
   if (s.tpi < s.lanes) s.tpi = s.lanes;
   while ((1 << s.log_tpi) < s.tpi) ++s.log_tpi;
   s.rows = s.tpi / s.lanes;
@@ -160,7 +164,7 @@ static bool divide_slab(const NormGeom& g, int64_t cv, int iters, Slab* out) {
   while ((1 << s.log_parts) < s.parts) ++s.log_parts;
   s.nb = 1;
   if (s.parts == 1)
-    while (s.nb * s.tpi < kSlabThreads && s.nb < g.B) s.nb *= 2;
+    while (s.nb * s.tpi < most_nb && s.nb < g.B) s.nb *= 2;
   s.img_blocks = (g.B + s.nb - 1) / s.nb;
   s.threads = s.nb * s.tpi < 64 ? 64 : s.nb * s.tpi;
   const int ppg = g.cg / g.q;
@@ -178,28 +182,38 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   const int64_t most = 16 * kSlabThreads, few = 4 * kSlabThreads;
   const bool small = (int64_t)g.B * g.P * g.nv < 256 * most;     // not enough to give every CU a full workgroup
   int64_t cv = g.nv <= 64 ? g.nv : unit * (64 / unit);
-  // fewer workgroups than CUs: narrower chunks, down to one line of 128 bytes per pixel
+  // Fewer workgroups than CUs: narrower chunks, down to one line of 128 bytes per pixel, or to 64 bytes where an image's
+  // chunk then has a workgroup of its own.  Measured, forward / backward: 8 images of 4x4x1024 fp32 4.0 / 7.0 us with whole
+  // pixels, 3.7 / 6.5 so; 32 of 16x16x64 bf16 6.0 / 11.3 with 128 bytes, 4.3 / 8.1 with 64 (with 32: 5.0 / 8.7); but
+  // 16 of 128x128x64 bf16, which have parts, 14.1 / 24.3 with 128 bytes and 18.8 / 38 with 64.
   for (;;) {
     const int64_t half = cv / 2 / unit * unit, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
-    if (half < 8 || wgs >= 256 || g.P * (int64_t)pow2_ceil(cv) <= 256) break;
+    const int64_t least = g.P * (int64_t)pow2_ceil(half) <= most ? 4 : 8;
+    if (half < least || wgs >= 256 || g.P * (int64_t)pow2_ceil(cv) <= 256) break;
     cv = half;
   }
-  // and below that, to two lanes' width or one, where it spares an image parts (and a launch)
-  if (small && g.P * (int64_t)pow2_ceil(cv) > most) {
+  // And below that, down to a lane, where it spares an image of a tensor of at most 256 KB its parts, whose words take a
+  // launch to empty: one image of 64x64x32 bf16 8.0 us forward and 11.1 backward on the device, with parts 8.0 and 11.7, and
+  // 3 us less on the host.  Larger tensors lose more by the lines read in pieces: one image of 64x64x64 11 and 23 us, with
+  // parts 7.7 and 11.5; 8 of 64x64x32 10.8 and 19.7, with parts 8.4 and 13.3.
+  if ((int64_t)g.B * g.P * g.nv <= 4 * most && g.P * (int64_t)pow2_ceil(cv) > most) {
     int64_t narrow = cv;
     while (narrow >= unit && g.P * (int64_t)pow2_ceil(narrow) > most) narrow = narrow / 2 / unit * unit;
     if (narrow >= unit) cv = narrow;
   }
   const int64_t vectors = (int64_t)g.P * pow2_ceil(cv);
-  // Up to 16 vectors a thread, as many as its registers hold, where that leaves every CU a workgroup.  Else 4, for a
-  // shorter time -- but not where that alone would split an image (parts cost a launch) or, backward, keep the images of
-  // a chunk from sharing a workgroup, which then needs no launch to join the parameter gradients.
+  // 16 vectors a thread, as many as its registers hold, where that leaves every CU a workgroup; else 4, and a fourth of the
+  // time.  An image of up to 4096 vectors then has up to 1024 threads, to be spared parts; backward, all images of a chunk
+  // share these threads if they can, and no launch has to join the parameter gradients.  Measured, forward / backward:
+  // 512 images of 4x4x256 bf16 4.5 / 10 us, with 16 vectors 6.2 / 15.2; 64 of 8x8x512 fp32 5.7 / 9.4 with 1024 threads,
+  // 6.6 / 11.3 with 16 vectors and 256; 8 of 4x4x1024 fp32 backward 4.7 and 6.5.
   const bool alone = backward && g.B <= kSlabThreads && pow2_ceil(g.B) * vectors <= most;
   int iters = small ? 4 : 16;
   if (vectors <= pow2_ceil(cv)) iters = 1;
-  else if (alone) iters = pow2_ceil(g.B) * vectors <= few ? 4 : 16;
-  else if (vectors > few && vectors <= most) iters = 16;
-  return divide_slab(g, cv, iters, out) || divide_slab(g, cv, 16, out);
+  else if (alone && pow2_ceil(g.B) * vectors <= few) iters = 4;
+  const int threads = small && vectors <= most ? kWideThreads : kSlabThreads;
+  return divide_slab(g, cv, iters, iters == 4 ? threads : kSlabThreads, alone && iters == 4 ? threads : kSlabThreads, out) ||
+         divide_slab(g, cv, 16, kSlabThreads, kSlabThreads, out);
 }
 static size_t slab_rows(const Slab& s) { return (size_t)s.img_blocks * s.parts; }   // rows of channel sums
 static size_t fwd_part_bytes(const NormGeom& g) { return (size_t)g.B * g.tiles * g.nv * g.n_slots * sizeof(float4); }
@@ -223,6 +237,13 @@ static int check_range(const NormGeom& g, const char* what) {
                  (int64_t)g.B * g.tiles * g.chunks < (1ll << 31), std::string(what) + ": tensor too large");
   return MI_OK;
 }
+// A launch holds less than 2^32 threads (one wave per image and group in the joins).
+static int check_threads(const NormGeom& g, const Slab* s, const char* what) {
+  const int64_t threads = s ? (int64_t)s->img_blocks * s->parts * s->chunks * s->threads
+                            : std::max((int64_t)g.B * g.tiles * g.chunks * kThreads, (int64_t)g.B * g.G * 64);
+  MI_REQUIRE(threads < (1ll << 32), std::string(what) + ": tensor too large");
+  return MI_OK;
+}
 int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, const float* beta, void* y, int ycs, int yco,
                           float* mean, float* rstd, int B, int H, int W, int C, int G, int act, float eps,
                           const mi_dropout* drop, int polls, void* ws, size_t ws_bytes, int dtype, hipStream_t s) {
@@ -234,6 +255,7 @@ int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, c
   if (B == 0) return MI_OK;
   Slab slab;
   const Slab* sl = choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, false, &slab) ? &slab : nullptr;
+  if ((rc = check_threads(a.g, sl, "group_norm_act_fwd"))) return rc;
   if (polls >= 0) slab.polls = polls;
   if (ws_bytes < group_norm_ws_bytes(B, H, W, C, G, 0, dtype)) return fail(MI_ESIZE, "group_norm_act_fwd: workspace too small");
   a.x = x; a.xcs = xcs; a.xco = xco;
@@ -253,15 +275,16 @@ int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int y
   if (rc) return rc;
   a.g = norm_geom(B, H, W, C, G, dtype);
   if ((rc = check_range(a.g, "group_norm_act_bwd"))) return rc;
+  Slab slab;
+  const Slab* sl = B > 0 && choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, true, &slab) ? &slab : nullptr;
+  if ((rc = check_threads(a.g, sl, "group_norm_act_bwd"))) return rc;
+  if (polls >= 0) slab.polls = polls;
   if (ws_bytes < group_norm_ws_bytes(B, H, W, C, G, 1, dtype)) return fail(MI_ESIZE, "group_norm_act_bwd: workspace too small");
   a.x = x; a.xcs = xcs; a.xco = xco;
   a.dy = dy; a.ycs = ycs; a.yco = yco;
   a.out = dx; a.ocs = dcs; a.oco = dco;
   a.gamma = gamma; a.beta = beta; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.act = act;
-  Slab slab;
-  const Slab* sl = B > 0 && choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, true, &slab) ? &slab : nullptr;
-  if (polls >= 0) slab.polls = polls;
   a.chan_stride = C;
   if (sl) {
     a.words = (uint64_t*)ws;

@@ -4,13 +4,19 @@
 //   dz = drop(dy) * act'(z),  t = gamma * dz,  dx = rstd * (t - mean_g(t) - h * mean_g(t * h))
 //   dgamma = sum dz * h,  dbeta = sum dz                                        over images and pixels
 //
-// Both directions are HBM-bound (about 10 and 40 operations per 4 and 6 bytes).  Everything is held in fp32 from the load on;
-// what is stored in bf16 is rounded once.
+// Everything is held in fp32 from the load on; what is stored in bf16 is rounded once.
 //
-// Tiles.  A workgroup owns kI * R pixels of one image and up to 64 vectors (16 bytes: 8 or 4 channels) of each: its
-// lanes lie along the channels, so a pixel's 64..1024 bytes are read by neighbours, and R = 256 / lanes-per-pixel rows
-// of pixels are read at a time.  A thread keeps its channels for all of its kI pixels: per-channel values are loaded
-// once and sums stay in registers until the end.
+// Two paths.  The slab kernels (below) read x, and backward dy, once into registers: one launch forward, and backward a
+// second for the parameter gradients where several workgroups hold rows of them.  They take every shape but images of more
+// than 64 parts (a part: at most 4096 vectors of up to 64 neighbouring ones per pixel) and groups that end together with a
+// vector only after more than 64 vectors.  Those take the general kernels, which read x (and dy) twice: sums of tiles, a join, a pass that applies.
+// Both are bound by HBM where a call is large, by the launches where it is small; the slab backward works for as long as
+// it loads (about 30 operations per value and 6 or 12 bytes).
+//
+// Tiles of the general kernels.  A workgroup owns kI * R pixels of one image and up to 64 vectors (16 bytes: 8 or 4
+// channels) of each: its lanes lie along the channels, so a pixel's 64..1024 bytes are read by neighbours, and R = 256 /
+// lanes-per-pixel rows of pixels are read at a time.  A thread keeps its channels for all of its kI pixels: per-channel
+// values are loaded once and sums stay in registers until the end.
 //
 // Precision of the statistics: the corrected two-pass form (Chan, Golub, LeVeque, "Algorithms for computing the sample
 // variance", 1983).  A tile's mean m comes first, from registers; then r = sum (x - m) and q = sum (x - m)^2, which give
@@ -33,7 +39,7 @@ struct NormGeom {
   int chunks;                  // ranges of `lanes` vectors that make up a pixel
   int rows;                    // pixels read at a time = kThreads / lanes
   int tiles;                   // per image
-  int q, n_slots;              // channels that are summed together, gcd(cg, vector width), and how often they fit a vector
+  int q, n_slots;              // channels that are summed together (a vector, 4 of a bf16 vector, or 1: must divide cg), pieces per vector
   FastDiv d_tiles, d_chunks, d_cg;
 };
 
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const NormArgs a) {
 //
 // A workgroup owns `nb` images x cv vectors.  Its threads are (image, row, lane): lanes lie along the channels, tpi
 // threads share an image.  A group's sum goes over the rows and lanes of a wave by shuffles and over waves through LDS.
-constexpr int kSlabThreads = 256;
+constexpr int kSlabThreads = 256, kWideThreads = 1024;
 struct Slab {
   int cv;                      // vectors per pixel of a chunk: whole groups
   int lanes, log_lanes;        // power of two >= cv, at most 64
@@ -549,7 +555,7 @@ __device__ __forceinline__ double parts_total(double v, const Slab& s) {
 // other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors: 16.3 us against 16.4
 // for 512 images of 32x32x32 forward, backward with 4 vectors 59 against 32).  128 registers: four workgroups a CU.
 template <typename T, int NS, int I, bool PARTS>
-__global__ __launch_bounds__(kSlabThreads, I > 4 ? 3 : 4) void gn_fwd_slab_kernel(const NormArgs a, const Slab s) {
+__global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I > 4 || PARTS ? 3 : 4) void gn_fwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   extern __shared__ float shared[];
   const NormGeom& g = a.g;
@@ -1073,7 +1079,7 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
 // group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
 // linear in it.
 template <typename T, int NS, int I, bool PARTS, int ACT>
-__global__ __launch_bounds__(kSlabThreads, I > 4 ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
+__global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I > 4 || PARTS ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N;
   extern __shared__ float shared[];
   const NormGeom& g = a.g;
