@@ -189,7 +189,7 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   for (;;) {
     const int64_t half = cv / 2 / unit * unit, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
     const int64_t least = g.P * (int64_t)pow2_ceil(half) <= most ? 4 : 8;
-    if (half < least || wgs >= 256 || g.P * (int64_t)pow2_ceil(cv) <= 256) break;
+    if (pow2_ceil(half) < least || wgs >= 256 || g.P * (int64_t)pow2_ceil(cv) <= 256) break;
     cv = half;
   }
   // And below that, down to a lane, where it spares an image of a tensor of at most 256 KB its parts, whose words take a

@@ -784,31 +784,43 @@ __global__ __launch_bounds__(kThreads) void gn_bwd_apply_kernel(const NormArgs a
 // ReLU's gate is a border that fp32 rounding of z may cross.  But z > 0 is  sign(gamma) x > sign(gamma) tau  with
 // tau = mean - beta / (rstd gamma), and x is an fp32 value: against tau in 64 bits, rounded down to fp32, the comparison is
 // exact.  A channel's tau is worked out once per workgroup; the gate costs two instructions and needs no z.
+// The quotient by two steps of Newton's method from the hardware's reciprocal (a library division works a special case per
+// operand out besides, one after the other).
 __device__ __forceinline__ float relu_threshold(float mean, float rstd, float gamma, float beta) {
-  if (gamma == 0.f) return beta > 0.f ? -INFINITY : INFINITY;
-  double tau = (double)mean - (double)beta / ((double)rstd * (double)gamma);
-  if (gamma < 0.f) tau = -tau;
+  const double d = (double)rstd * (double)gamma;                 // 48 bits: exact
+  double r = __builtin_amdgcn_rcp(d);
+  r = fma(fma(-d, r, 1.0), r, r);
+  r = fma(fma(-d, r, 1.0), r, r);
+  double tau = fma(-(double)beta, r, (double)mean);
+  tau = gamma < 0.f ? -tau : tau;
   const float f = (float)tau;
-  return (double)f > tau ? nextafterf(f, -INFINITY) : f;
+  const float below = f > 0.f ? __uint_as_float(__float_as_uint(f) - 1) : __uint_as_float(f < 0.f ? __float_as_uint(f) + 1 : 0x80000001u);
+  const float t = (double)f > tau ? below : f;                   // f itself where tau is an fp32 value, infinite or NaN
+  return gamma == 0.f ? (beta > 0.f ? -INFINITY : INFINITY) : t;
 }
 __device__ __forceinline__ bool relu_gate(float x, float gamma, float threshold) {
   return __uint_as_float(__builtin_amdgcn_bitop3_b32(__float_as_uint(x), __float_as_uint(gamma), 0x80000000u, 0x78)) > threshold;   // x ^ (gamma & sign)
 }
-// The thresholds of a thread's channels, through LDS (nb * lanes * N floats).  `first` brings a thread's first channel: it is
-// read before the tile's loads are issued, which complete in order.
+// The thresholds of a thread's channels.  At least N rows of threads share the work: a thread does one at most, they pass
+// through LDS (nb * lanes * N floats), and `first`, what it is made of, is read before the tile's loads are issued, which
+// complete in order.  Fewer rows: every thread its own, from its channels' values (512 images of 2x2x512 bf16 backward
+// 11.9 us where they shared it and fetched what the further ones are made of, 9.6 so).
 struct ReluInputs { float mean, rstd, gamma, beta; };
 __device__ __forceinline__ ReluInputs relu_inputs(const NormArgs& a, const SlabThread& t, int c0, int k) {
   const int c = min(c0 + k, a.g.C - 1);
   const int64_t gi = (int64_t)t.b * a.g.G + fdiv((uint32_t)c, a.g.d_cg);
   return ReluInputs{a.mean[gi], a.rstd[gi], a.gamma ? a.gamma[c] : 1.f, a.beta ? a.beta[c] : 0.f};
 }
-template <int N>
-__device__ __forceinline__ void relu_thresholds(const NormArgs& a, const Slab& s, const SlabThread& t, ReluInputs first, float* shared, float* out) {
-  float* mine = shared + t.slot * s.lanes * N;
-  for (int k = t.tin; k < s.lanes * N; k += s.tpi) {
-    const ReluInputs r = k == t.tin ? first : relu_inputs(a, t, t.chunk * s.cv * N, k);
-    mine[k] = relu_threshold(r.mean, r.rstd, r.gamma, r.beta);
+template <int NS, int N>
+__device__ __forceinline__ void relu_thresholds(const Slab& s, const SlabThread& t, ReluInputs first, const float* mean, const float* rstd,
+                                                const float* gamma, const float* beta, float* shared, float* out) {
+  if (s.rows < N) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = relu_threshold(mean[j * NS / N], rstd[j * NS / N], gamma[j], beta[j]);
+    return;
   }
+  float* mine = shared + t.slot * s.lanes * N;
+  if (t.tin < s.lanes * N) mine[t.tin] = relu_threshold(first.mean, first.rstd, first.gamma, first.beta);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < N; ++j) out[j] = mine[t.lane * N + j];
@@ -931,8 +943,9 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
   const int c0 = opaque(t.v * N), chunk_c0 = t.chunk * s.cv * N;
   float mean[NS], rstd[NS], scaled[N], beta[N], threshold[N], ch[2 * N] = {}, sum[2][NS];
   slab_channels<NS, N>(a, t.b, c0, mean, rstd, scaled, beta);
+  if constexpr (ACT == MI_ACT_RELU)
+    relu_thresholds<NS, N>(s, t, relu_inputs(a, t, chunk_c0, t.tin), mean, rstd, scaled, beta, shared, threshold);
   slab_scale<NS, N>(rstd, scaled);
-  if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, relu_inputs(a, t, chunk_c0, t.tin), shared, threshold);
   const auto x = in_memory<T, I>(t, px, g, s, a.x, a.xcs, a.xco), dy = in_memory<T, I>(t, px, g, s, a.dy, a.ycs, a.yco);
 #pragma unroll 1
   for (int i = 0; i < I; ++i) {
@@ -1094,7 +1107,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
   slab_channels<NS, N>(a, t.b, c0, mean, rstd, scaled, beta);
   load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, vx);
   load_slab<T, I>(t, px, g, s, a.dy, a.ycs, a.yco, vd);
-  if constexpr (ACT == MI_ACT_RELU) relu_thresholds<N>(a, s, t, first, shared, threshold);
+  if constexpr (ACT == MI_ACT_RELU) relu_thresholds<NS, N>(s, t, first, mean, rstd, scaled, beta, shared, threshold);
   slab_scale<NS, N>(rstd, scaled);
   bwd_drop<T, I>(a, s, t, px, vd);
   zero_missing(px, vx);
