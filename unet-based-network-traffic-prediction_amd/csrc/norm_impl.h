@@ -552,8 +552,13 @@ __device__ __forceinline__ double parts_total(double v, const Slab& s) {
 }
 
 // 256 threads with up to 16 vectors each: what a thread does once -- its place, its channels' parameters, the sums over
-// other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors: 16.3 us against 16.4
-// for 512 images of 32x32x32 forward, backward with 4 vectors 59 against 32).  128 registers: four workgroups a CU.
+// other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors, forward: 16.3 us
+// against 16.4 for 512 images of 32x32x32 bf16).  16 vectors leave three workgroups a CU (up to 168 registers); 4 vectors
+// stay within 128, so 1024 threads fit.
+// Bound by HBM: 1024 images of 64x64x32 bf16 with SiLU, four parts each, 98 us for 537 MB = 5.5 TB/s, and 2 us for the launch
+// that empties the words; 512 of 32x32x32 with ReLU and dropout 10 % 14.3 us for 67 MB = 4.7 TB/s (the mask's words are
+// worked out while the loads are in flight).  One image of 64x64x32: 8 us, of which a launch is 2.8 and the rest one
+// memory latency after the other.
 template <typename T, int NS, int I, bool PARTS>
 __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I > 4 || PARTS ? 3 : 4) void gn_fwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
@@ -1091,6 +1096,11 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
 // One read of x and dy: the same division of the work as forward.  Sums of dz and dz * h for each channel come first; a
 // group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
 // linear in it.
+// 16 vectors of x and of dy take 128 registers, all of it up to 256: two workgroups a CU.  Those load together, compute
+// together and store together, so the time is near the sum of both: 64 images of 128x128x32 bf16 with SiLU 51 us for 201 MB
+// (32 of memory at 6.2 TB/s; about 4700 instructions a wave, 27 us), 512 of 32x32x32 with ReLU and dropout 20 for 101 MB.
+// What did not help there: 8 vectors a thread and three workgroups, a staggered start, workgroups that stay and prefetch
+// the next part (their polls and stores queue behind the prefetch: 83 us against 62), loads of x and dy in turn.
 template <typename T, int NS, int I, bool PARTS, int ACT>
 __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I > 4 || PARTS ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N;
