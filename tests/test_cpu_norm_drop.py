@@ -104,6 +104,16 @@ def test_c_refusals(ua):
     assert _norm_bwd(L, dy=A << 9, dx=A << 10, B=300, H=40, W=40, ws_bytes=8) == -2 and b"workspace" in L.mi_last_error()
 
 
+def test_more_threads_than_a_launch_holds_are_refused(ua):
+    L = ua.lib()
+    far = 1 << 45                                                 # behind a tensor of 2^30 pixels
+    for call in (lambda: _norm_fwd(L, B=1 << 30, H=1, W=1, Cc=64, G=8, y=far, dt=1),
+                 lambda: _norm_bwd(L, B=1 << 30, H=1, W=1, Cc=64, G=8, dy=far, dx=far << 1, ws_bytes=1 << 60),
+                 lambda: _norm_fwd(L, B=1 << 26, H=1, W=1, Cc=640, G=1, xcs=640, ycs=640, y=far, ws_bytes=1 << 60),
+                 lambda: _drop(L, B=1 << 30, H=1, W=1, Cc=256, xcs=256, ycs=256, y=far)):
+        assert call() == -1 and b"too large" in L.mi_last_error()
+
+
 def test_empty_batches_need_nothing(ua):
     L = ua.lib()
     assert _norm_fwd(L, B=0, x=None, y=None, mean=None, rstd=None, ws=None) == 0

@@ -525,6 +525,48 @@ def test_streams_and_graph_replay(ua):
         assert all(torch.equal(s, t) for s, t in zip(out, eager(n))), n
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_shared_images_on_two_streams_and_in_graphs(ua, dtype):
+    """Images that several workgroups share: calls on two streams at once, and captured calls whose inputs change between
+    replays (what the workgroups told each other in the replay before is then wrong)."""
+    ops = ua.ops
+    B, H, W, C, G = 5, 120, 110, 64, 8
+    inputs = [(place(rnd(i, B, H, W, C, shift=float(i)), dtype), place(rnd(10 + i, B, H, W, C), dtype)) for i in range(3)]
+    w, b = rnd(3, C, shift=1.0).cuda(), rnd(4, C).cuda()
+    drop = ops.Drop(0.3, 5)
+
+    def train(x, dy):
+        y, m, r = ops.group_norm_act_fwd(x, C, G, w, b, act="silu", drop=drop)
+        return (y, m, r) + ops.group_norm_act_bwd(x, dy, m, r, C, G, w, b, act="silu", drop=drop)
+    want = [train(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for n in range(6):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(train(*inputs[(n + k) % 3]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for n, out in enumerate(got[k]):
+            assert all(torch.equal(s, t) for s, t in zip(out, want[(n + k) % 3])), (k, n)
+    x, dy = (t.clone() for t in inputs[0])
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0][0].pool() if graphs else None):
+            out = train(x, dy)
+        graphs.append((g, out))
+    for n in range(6):
+        g, out = graphs[n % 2]
+        x.copy_(inputs[n % 3][0])
+        dy.copy_(inputs[n % 3][1])
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(s, t) for s, t in zip(out, want[n % 3])), n
+        train(*inputs[(n + 1) % 3])
+
+
 def test_captured_autograd_step(ua):
     """Forward and backward of the modules captured through autograd, leaves' gradients and all."""
     C, G = 64, 8
