@@ -124,9 +124,22 @@ template <> struct ActVec<__bf16> {
 #pragma unroll
     for (int j = 0; j < 2; ++j) v[2 * h + j] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)f[2 * j], (__bf16)f[2 * j + 1]});
   }
-  static __device__ __forceinline__ void pack4_exact(const float* f, int h, u32x4_t& v) {   // of values that are bf16 already
+  static __device__ __forceinline__ void pack4_exact(const float* f, int h, u32x4_t& v) {   // the upper halves: of values that are bf16 already, all of them
 #pragma unroll
     for (int j = 0; j < 2; ++j) v[2 * h + j] = __builtin_amdgcn_perm(__float_as_uint(f[2 * j + 1]), __float_as_uint(f[2 * j]), 0x07060302);
+  }
+  // fp32 values as two vectors of 16-bit halves
+  static __device__ __forceinline__ void split4(const float* f, int h, u32x4_t& high, u32x4_t& low) {
+    pack4_exact(f, h, high);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) low[2 * h + j] = __builtin_amdgcn_perm(__float_as_uint(f[2 * j + 1]), __float_as_uint(f[2 * j]), 0x05040100);
+  }
+  static __device__ __forceinline__ void join4(u32x4_t high, u32x4_t low, int h, float* f) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      f[2 * j] = __uint_as_float(__builtin_amdgcn_perm(high[2 * h + j], low[2 * h + j], 0x05040100));
+      f[2 * j + 1] = __uint_as_float(__builtin_amdgcn_perm(high[2 * h + j], low[2 * h + j], 0x07060302));
+    }
   }
   static __device__ __forceinline__ void unpack(u32x4_t v, float* f) {
     unpack4(v, 0, f);

@@ -897,10 +897,10 @@ __device__ __forceinline__ void store_channel(const NormArgs& a, int row, int c,
   if (a.dbeta) a.dbeta[c] = a.ga * sum_dz + (a.gb != 0.f ? a.gb * a.dbeta[c] : 0.f);
 }
 // Adds a vector's dz and dz * (x - mean) to the sums of its channels (d4: dy, dropped units cleared; scaled: gamma * rstd).
-// What the second pass needs of dy comes back: with gated-off units cleared, in fp32 as dz itself (a bf16 dz would be
-// rounded: its slope is worked out again).
-template <typename T, int NS, int ACT>
-__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const float* mean, const float* scaled, const float* beta,
+// What the second pass needs of dy comes back: with gated-off units cleared; in fp32 as dz itself, and so in bf16 with
+// SPLIT, the upper halves of dz in d4, the lower ones in `low` (else its slope is worked out again: a bf16 dz would be rounded).
+template <typename T, int NS, int ACT, bool SPLIT>
+__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, u32x4_t& low, const float* mean, const float* scaled, const float* beta,
                                          const float* threshold, float* ch) {
   constexpr int N = ActVec<T>::N;
 #pragma unroll
@@ -921,6 +921,13 @@ __device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, const float* m
       for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[4 * e + j], beta[4 * e + j]));
     }
     if constexpr (N == 4 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) ActVec<T>::pack4(d, e, d4);
+    if constexpr (SPLIT) {
+      ActVec<T>::split4(d, e, d4, low);
+      if (e == N / 4 - 1) {
+        pin(d4, mean[0]);
+        pin(low, mean[0]);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       ch[4 * e + j] += d[j];
@@ -961,7 +968,8 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
       keep.add(0, a.drop, drop_offset(a.drop), row * (uint32_t)(g.nv * N) + c0);
       d = keep.kept(0, d);
     }
-    bwd_step<T, NS, ACT>(x(i, 0.f), d, mean, scaled, beta, threshold, ch);
+    u32x4_t unused;
+    bwd_step<T, NS, ACT, false>(x(i, 0.f), d, unused, mean, scaled, beta, threshold, ch);
   }
   bwd_group_sums<NS, N>(ch, scaled, sum);
   slab_sum<NS, 2>(sum, g, s, t, shared);
@@ -1049,9 +1057,9 @@ __device__ __forceinline__ void bwd_means(const NormArgs& a, const Slab& s, cons
 }
 // dx of a part from the registers:  dx = scaled * dz - M1 - (x - mean) * rstd^2 * M2,  M1 and M2 the means over the group of
 // scaled * dz and scaled * dz * (x - mean); times dropout's factor.
-template <typename T, int NS, int I, int ACT>
+template <typename T, int NS, int I, int ACT, bool SPLIT>
 __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const SlabThread& t, const SlabPixels& px, u32x4_t (&vx)[I],
-                                         u32x4_t (&vd)[I], const float* mean, const float* rstd, const float* scaled, const float* beta,
+                                         u32x4_t (&vd)[I], const u32x4_t* low, const float* mean, const float* rstd, const float* scaled, const float* beta,
                                          const float (&sum)[2][NS], float factor) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   const int c0 = t.v * N;
@@ -1071,16 +1079,19 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
   for (int i = 0; i < I; ++i) {
     pin(vx[i], sum[0][0]);
     pin(vd[i], sum[0][0]);
+    u32x4_t lo;
+    if constexpr (SPLIT) lo = low[i * kSlabThreads];
 #pragma unroll
     for (int e = 0; e < N / 4; ++e) {
       float x[4], d[4];
       ActVec<T>::unpack4(vx[i], e, x);
-      ActVec<T>::unpack4(vd[i], e, d);
+      if constexpr (SPLIT) ActVec<T>::join4(vd[i], lo, e, d);
+      else ActVec<T>::unpack4(vd[i], e, d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = 4 * e + j, k = c / Q;
         x[j] -= mean[k];
-        if constexpr (N == 8 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[c], beta[c]));
+        if constexpr (N == 8 && !SPLIT && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[c], beta[c]));
         d[j] = fmaf(x[j], b1[k], fmaf(d[j], slope[c], b0[k]));
       }
       if (ragged) {
@@ -1104,7 +1115,9 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
 template <typename T, int NS, int I, bool PARTS, int ACT>
 __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I > 4 || PARTS ? 2 : 4) void gn_bwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N;
+  constexpr bool SPLIT = N == 8 && NS < N && I == 16 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU);
   extern __shared__ float shared[];
+  __shared__ u32x4_t low[SPLIT ? I * kSlabThreads : 1];          // [vector][thread]: each thread's own
   const NormGeom& g = a.g;
   const SlabThread t = slab_thread(g, s);
   const int c0 = t.v * N;
@@ -1126,7 +1139,9 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
   for (int i = 0; i < I; ++i) {
     pin(vx[i], scaled[0]);
     pin(vd[i], scaled[0]);
-    bwd_step<T, NS, ACT>(vx[i], vd[i], mean, scaled, beta, threshold, ch);
+    u32x4_t lo;
+    bwd_step<T, NS, ACT, SPLIT>(vx[i], vd[i], lo, mean, scaled, beta, threshold, ch);
+    if constexpr (SPLIT) low[i * kSlabThreads + threadIdx.x] = lo;
   }
   bwd_group_sums<NS, N>(ch, scaled, sum);
   slab_sum<NS, 2>(sum, g, s, t, shared);
@@ -1139,7 +1154,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
     slab_channels<NS, N>(a, t.b, opaque(c0), mean, rstd, scaled, beta);
     slab_scale<NS, N>(rstd, scaled);
   }
-  bwd_emit<T, NS, I, ACT>(a, s, t, px, vx, vd, mean, rstd, scaled, beta, sum, scale);
+  bwd_emit<T, NS, I, ACT, SPLIT>(a, s, t, px, vx, vd, low + threadIdx.x, mean, rstd, scaled, beta, sum, scale);
 }
 // ---------------------------------------------------------------- launches
 // in norm.hip
