@@ -110,6 +110,7 @@ SHAPES = [  # B, H, W, C, groups
     (2, 70, 67, 36, 9), (5, 5, 5, 100, 25), (130, 2, 2, 48, 3), (1, 128, 128, 32, 8), (1, 7, 1, 528, 1), (2, 6, 6, 2080, 13),
     (1, 200, 210, 24, 2), (17, 16, 16, 128, 32), (18, 64, 64, 64, 32), (9, 64, 60, 48, 6), (33, 20, 20, 96, 12),
     (257, 7, 7, 512, 8), (8, 4, 4, 1024, 32), (7, 23, 23, 96, 8), (3, 64, 64, 64, 8), (5, 16, 16, 64, 8), (40, 7, 5, 56, 56),
+    (1, 130, 255, 100, 20), (1, 256, 255, 66, 3),
 ]
 
 
@@ -287,6 +288,27 @@ def test_sums_of_parts_that_have_not_come(ua, monkeypatch, dtype, kind):
             got = (y, m, r) + ops.group_norm_act_bwd(x, dy, m, r, C, G, w, b, act=kind, drop=drop)
             assert all(torch.equal(s, t) for s, t in zip(want, got)), (B, H, W, C, G)
         monkeypatch.setattr(ops, "_POLLS", -1)
+
+
+def test_workgroups_that_share_an_image_run_together(ua, monkeypatch):
+    """More workgroups than can run at a time, in many chunks and parts: none may wait for one that comes much later (then
+    a call takes as long as their patience, 0.3 s; together they take 0.2 ms)."""
+    ops = ua.ops
+    B, H, W, C, G = 3, 128, 128, 1024, 1024
+    gen = torch.Generator("cuda").manual_seed(1)
+    x, dy = (torch.randn(B, H, W, C, device="cuda", generator=gen) for _ in range(2))
+    for _ in range(3):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        y, m, r = ops.group_norm_act_fwd(x, C, G, act="relu")
+        dx, _, _ = ops.group_norm_act_bwd(x, dy, m, r, C, G, act="relu")
+        end.record()
+        torch.cuda.synchronize()
+    assert start.elapsed_time(end) < 30.0
+    monkeypatch.setattr(ops, "_POLLS", 0)
+    z, m2, r2 = ops.group_norm_act_fwd(x, C, G, act="relu")
+    assert torch.equal(y, z) and torch.equal(m, m2) and torch.equal(r, r2)
+    assert torch.equal(dx, ops.group_norm_act_bwd(x, dy, m, r, C, G, act="relu")[0])
 
 
 def test_gradient_against_differences(ua):

@@ -186,10 +186,15 @@ static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   // chunk then has a workgroup of its own.  Measured, forward / backward: 8 images of 4x4x1024 fp32 4.0 / 7.0 us with whole
   // pixels, 3.7 / 6.5 so; 32 of 16x16x64 bf16 6.0 / 11.3 with 128 bytes, 4.3 / 8.1 with 64 (with 32: 5.0 / 8.7); but
   // 16 of 128x128x64 bf16, which have parts, 14.1 / 24.3 with 128 bytes and 18.8 / 38 with 64.
+  // Backward, an image of more than 64 parts is cut into narrower chunks whatever their number: one of 256x256x512 fp32 616 us
+  // by the general kernels, 151 in chunks of 64 bytes, 16 of 256x256x64 bf16 225 and 124; forward 120 and 146, 88 and 106.
   for (;;) {
-    const int64_t half = cv / 2 / unit * unit, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
-    const int64_t least = g.P * (int64_t)pow2_ceil(half) <= most ? 4 : 8;
-    if (pow2_ceil(half) < least || wgs >= 256 || g.P * (int64_t)pow2_ceil(cv) <= 256) break;
+    const int64_t lanes = pow2_ceil(cv), size = g.P * lanes, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
+    int64_t half = cv / 2 / unit * unit;
+    if (2 * pow2_ceil(half) < lanes) half = lanes / 2 / unit * unit;
+    const bool cut = backward && size > kMaxParts * most;
+    const int64_t least = cut || g.P * (int64_t)pow2_ceil(half) <= most ? 4 : 8;
+    if (pow2_ceil(half) < least || (!cut && (wgs >= 256 || size <= 256))) break;
     cv = half;
   }
   // And below that, down to a lane, where it spares an image of a tensor of at most 256 KB its parts, whose words take a
