@@ -141,7 +141,7 @@ static int pow2_ceil(int64_t v) {
   return p;
 }
 // How the slab kernels divide the work, or false where they do not apply.
-// Up to 64 parts: the lanes of the wave that joins them.  Without parts, by the general kernels: 16 images of 128x128x64
+// Up to 64 parts, which run at the same time on a fraction of the card.  Without parts, by the general kernels: 16 images of 128x128x64
 // bf16 20 us forward and 75 backward, with them 14 and 25; 2 of 256x256x32 12.7 and 50 against 13.6 and 20.
 constexpr int kMaxParts = 64;
 constexpr int kPolls = 4096;                 // about 1 us each
@@ -161,7 +161,6 @@ static bool divide_slab(const NormGeom& g, int64_t cv, int iters, int most, int 
   const int64_t parts = (g.P + (int64_t)s.rows * iters - 1) / ((int64_t)s.rows * iters);
   if (parts > kMaxParts) return false;
   s.parts = (int)parts;
-  while ((1 << s.log_parts) < s.parts) ++s.log_parts;
   s.nb = 1;
   if (s.parts == 1)
     while (s.nb * s.tpi < most_nb && s.nb < g.B) s.nb *= 2;

@@ -290,7 +290,7 @@ struct Slab {
   int tpi, log_tpi;            // threads per image, a power of two >= lanes
   int nb, img_blocks;          // images per workgroup, workgroups along the images
   int rows;                    // tpi / lanes
-  int parts, log_parts;        // workgroups that share an image (then nb = 1); rounded up to a power of two
+  int parts;                   // workgroups that share an image (then nb = 1, tpi = kSlabThreads)
   int merge;                   // lanes of a group that shuffles can sum (a power of two), ...
   int left;                    // ... and what then remains: pieces per group / merge
   int threads, iters;          // nb * tpi, pixels per thread
@@ -510,34 +510,72 @@ __device__ __forceinline__ void put_word(uint64_t* p, uint64_t w) { __hip_atomic
 __device__ __forceinline__ uint64_t get_word(const uint64_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// Runs `take(group of the chunk, present, first word, last word)` for every (group, part) of the workgroup's image, lane
-// % 2^log_parts = part, once all W words of all parts are there.  Returns the number of a missing part, or -1.
-template <int W, typename F>
-__device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeom& g, const Slab& s, const SlabThread& t, int groups,
-                                            int* missing, F take) {
-  const int tid = threadIdx.x, lane = tid & 63, per_wave = 64 >> s.log_parts;
+// For each group of the chunk: `term(part, first word, last word, part 0's first word, s0, s1)` adds a part to two sums, over all
+// parts in an order that depends on their number alone, and `take(group, s0, s1, part 0's first word)` gets these.  Returns the
+// number of a part that has not come, or -1.
+// Threads are (share of the parts, group), up to 64 groups at a time, so that the words of several parts are under way together
+// and few sums cross lanes (with the parts along a wave's lanes and one group after the other, 64 images of 100x100x64 fp32 in
+// 64 groups took 116 us forward and 127 backward, so 91 and 106).
+template <int W, typename Term, typename Take>
+__device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeom& g, const Slab& s, int groups, int* missing,
+                                            double2* partial, Term term, Take take) {
+  constexpr int U = 4, kWavesOfPart = kSlabThreads / 64;
+  const int tid = threadIdx.x, log_w = groups > 1 ? 32 - __clz(min(groups, 64) - 1) : 0, width = 1 << log_w;
+  const int own = tid & (width - 1), share = tid >> log_w, shares = kSlabThreads >> log_w;
+  bool failed = false;
   if (tid == 0) *missing = -1;
   __syncthreads();
-  const int part = lane & ((1 << s.log_parts) - 1);
-  for (int k = (tid >> 6) * per_wave; k < groups; k += (s.threads >> 6) * per_wave) {
-    const int group = k + (lane >> s.log_parts);
-    const bool needed = part < s.parts && group < groups;
-    const uint64_t* w = words + W * ((int64_t)min(part, s.parts - 1) * g.G + min(group, groups - 1));
-    uint64_t a = kEmpty, b = kEmpty;
-    for (int i = 0;; ++i) {
-      a = get_word(w);
-      b = W == 2 ? get_word(w + 1) : 0;
-      const bool there = !needed || (a != kEmpty && b != kEmpty);
-      if (__all(there)) break;
-      if (i >= s.polls) {
-        if (!there) atomicMax(missing, part);
-        break;
+  for (int base = 0; base < groups; base += width) {
+    const bool real = base + own < groups;
+    const uint64_t* w = words + W * min(base + own, groups - 1);
+    uint64_t first = 0, a[U], b[U];
+    double s0 = 0.0, s1 = 0.0;
+    for (int p0 = share; p0 - share < s.parts && !failed; p0 += shares * U) {
+      for (int i = 0;; ++i) {
+        bool all = true;
+        if constexpr (W == 2) {
+          first = get_word(w);
+          all = !real || first != kEmpty;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int p = p0 + u * shares;
+          const uint64_t* at = w + W * ((int64_t)min(p, s.parts - 1) * g.G);
+          a[u] = get_word(at);
+          b[u] = W == 2 ? get_word(at + 1) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) all = all && (!real || p0 + u * shares >= s.parts || (a[u] != kEmpty && b[u] != kEmpty));
+        if (__all(all)) break;
+        if (i >= s.polls) {
+          if (real && W == 2 && first == kEmpty) atomicMax(missing, 0);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (real && p0 + u * shares < s.parts && (a[u] == kEmpty || b[u] == kEmpty)) atomicMax(missing, p0 + u * shares);
+          failed = true;
+          break;
+        }
+        __builtin_amdgcn_s_sleep(1);
       }
-      __builtin_amdgcn_s_sleep(1);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p0 + u * shares < s.parts) term(p0 + u * shares, a[u], b[u], first, s0, s1);
     }
-    take(group, needed, a, b);
+    for (int o = 32; o >= width; o >>= 1) {
+      s0 += __shfl_xor(s0, o, 64);
+      s1 += __shfl_xor(s1, o, 64);
+    }
+    if ((tid & 63) < width) partial[(tid >> 6) * width + own] = make_double2(s0, s1);
+    __syncthreads();
+    if (tid < width && real) {
+      for (int k = 1; k < kWavesOfPart; ++k) {
+        s0 += partial[k * width + own].x;
+        s1 += partial[k * width + own].y;
+      }
+      take(base + own, s0, s1, first);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const int result = *missing;
   __syncthreads();
   return result;
@@ -546,11 +584,10 @@ __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeo
 template <int NS> __device__ __forceinline__ int slab_stats_at(const Slab& s) {
   return s.tpi <= 64 && s.left == 1 ? 0 : ((s.threads + 63) >> 6) * s.lanes * 2 * NS;
 }
-// Sum over the lanes that hold the parts of one group.
-__device__ __forceinline__ double parts_total(double v, const Slab& s) {
-  for (int o = (1 << s.log_parts) >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
+// Behind them, the number of a missing part, and the sums of the waves.
+constexpr int kPartialFloats = kSlabThreads * 4;
+__device__ __forceinline__ int* missing_at(float* stats, int groups) { return (int*)(stats + 2 * groups); }
+__device__ __forceinline__ double2* partial_at(float* stats, int groups) { return (double2*)(stats + ((2 * groups + 5) & ~3)); }
 
 // 256 threads with up to 16 vectors each: what a thread does once -- its place, its channels' parameters, the sums over
 // other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors, forward: 16.3 us
@@ -612,17 +649,19 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
     };
     publish(t.part);
     for (;;) {
-      const int part = slab_collect<2>(words, g, s, t, groups, (int*)(stats + 2 * groups), [&](int group, bool there, uint64_t w0, uint64_t w1) {
-        const int p = threadIdx.x & ((1 << s.log_parts) - 1);
-        const double n = there ? (double)min(g.P - p * s.rows * I, s.rows * I) * g.cg : 0.0;
-        const double m = there ? __longlong_as_double((long long)w0) : 0.0, dev = there ? __longlong_as_double((long long)w1) : 0.0;
-        const double all = (double)g.P * g.cg, mu = parts_total(n * m, s) / all, d = m - mu;
-        const double var = parts_total(dev + n * d * d, s) / all;
-        if (p == 0 && there) {
-          stats[2 * group] = (float)mu;
+      // deviations from part 0's mean: those of the means themselves, so nothing cancels that 64 bits would miss
+      const int part = slab_collect<2>(words, g, s, groups, missing_at(stats, groups), partial_at(stats, groups),
+        [&](int p, uint64_t w0, uint64_t w1, uint64_t first, double& s0, double& s1) {
+          const double n = (double)min(g.P - p * s.rows * I, s.rows * I) * g.cg;
+          const double d = __longlong_as_double((long long)w0) - __longlong_as_double((long long)first);
+          s0 = fma(n, d, s0);
+          s1 += fma(n * d, d, __longlong_as_double((long long)w1));
+        },
+        [&](int group, double s0, double s1, uint64_t first) {
+          const double all = (double)g.P * g.cg, d = s0 / all, var = s1 / all - d * d;
+          stats[2 * group] = (float)(__longlong_as_double((long long)first) + d);
           stats[2 * group + 1] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)a.eps));
-        }
-      });
+        });
       if (__builtin_expect(part < 0, 1)) break;
       const SlabPixels other = slab_pixels<I>(t, g, s, part);
       slab_moments<T, NS, I>(in_memory<T, I>(t, other, g, s, a.x, a.xcs, a.xco), other, g, s, t, shared, mean, e, q);
@@ -1035,16 +1074,16 @@ __device__ __forceinline__ void bwd_means(const NormArgs& a, const Slab& s, cons
     float* stats = shared + slab_stats_at<NS>(s);
     __syncthreads();
     for (;;) {
-      const int part = slab_collect<1>(words, g, s, t, groups, (int*)(stats + 2 * groups), [&](int group, bool there, uint64_t w, uint64_t) {
-        const int p = threadIdx.x & ((1 << s.log_parts) - 1);
-        const double n = (double)g.P * g.cg;
-        const double m1 = parts_total(there ? (double)__uint_as_float((uint32_t)w) : 0.0, s) / n;
-        const double m2 = parts_total(there ? (double)__uint_as_float((uint32_t)(w >> 32)) : 0.0, s) / n;
-        if (p == 0 && there) {
-          stats[2 * group] = (float)m1;
-          stats[2 * group + 1] = (float)m2;
-        }
-      });
+      const int part = slab_collect<1>(words, g, s, groups, missing_at(stats, groups), partial_at(stats, groups),
+        [&](int, uint64_t w, uint64_t, uint64_t, double& s0, double& s1) {
+          s0 += (double)__uint_as_float((uint32_t)w);
+          s1 += (double)__uint_as_float((uint32_t)(w >> 32));
+        },
+        [&](int group, double s0, double s1, uint64_t) {
+          const double n = (double)g.P * g.cg;
+          stats[2 * group] = (float)(s0 / n);
+          stats[2 * group + 1] = (float)(s1 / n);
+        });
       if (__builtin_expect(part < 0, 1)) break;
       bwd_other_part<T, NS, I, ACT>(a, s, t, part, shared);
     }
@@ -1178,7 +1217,7 @@ template <typename T, int NS>
 void launch_fwd_slab(const NormArgs& a, const Slab& sl, hipStream_t s) {
   const dim3 grid(slab_grid(sl)), block((unsigned)sl.threads);
   // the sums, and with several parts (mean, rstd) of each group of the chunk and a number
-  const int floats = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 : 0);
+  const int floats = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 + kPartialFloats : 0);
   const unsigned lds = (unsigned)(floats * sizeof(float));
   if (sl.parts > 1) launch_gn_empty(a.words, slab_words(a.g, sl), s);
 #define GN_SLAB(I, PARTS) hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, I, PARTS>), grid, block, lds, s, a, sl)
@@ -1221,7 +1260,7 @@ void launch_bwd_slab_act(const NormArgs& a, const Slab& sl, dim3 grid, dim3 bloc
 template <typename T, int NS>
 void launch_bwd_slab(const NormArgs& a, const Slab& sl, hipStream_t s) {
   const dim3 grid(slab_grid(sl)), block((unsigned)sl.threads);
-  const int sums = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 : 0);
+  const int sums = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 + kPartialFloats : 0);
   const int channels = a.dgamma || a.dbeta ? (sl.threads >> 6) * sl.lanes * 2 * ActVec<T>::N : 0;
   const int thresholds = a.act == MI_ACT_RELU ? (sl.threads >> sl.log_tpi) * sl.lanes * ActVec<T>::N : 0;
   int floats = sums > channels ? sums : channels;
