@@ -10,8 +10,8 @@
 // second for the parameter gradients where several workgroups hold rows of them.  They take every shape but images of more
 // than 64 parts (a part: at most 4096 vectors of up to 64 neighbouring ones per pixel) and groups that end together with a
 // vector only after more than 64 vectors.  Those take the general kernels, which read x (and dy) twice: sums of tiles, a join, a pass that applies.
-// Both are bound by HBM where a call is large, by the launches where it is small; the slab backward works for as long as
-// it loads (about 30 operations per value and 6 or 12 bytes).
+// Both are bound by HBM where a call is large, by the launches where it is small; the slab backward works nearly as long
+// as it loads (about 20 operations per value, of 6 or 12 bytes, and twice that with dropout).
 //
 // Tiles of the general kernels.  A workgroup owns kI * R pixels of one image and up to 64 vectors (16 bytes: 8 or 4
 // channels) of each: its lanes lie along the channels, so a pixel's 64..1024 bytes are read by neighbours, and R = 256 /
@@ -540,9 +540,11 @@ __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeo
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int p = p0 + u * shares;
+          a[u] = b[u] = 0;
+          if (p - share >= s.parts) continue;                    // uniform: nobody has that many
           const uint64_t* at = w + W * ((int64_t)min(p, s.parts - 1) * g.G);
           a[u] = get_word(at);
-          b[u] = W == 2 ? get_word(at + 1) : 0;
+          if (W == 2) b[u] = get_word(at + 1);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) all = all && (!real || p0 + u * shares >= s.parts || (a[u] != kEmpty && b[u] != kEmpty));
@@ -593,7 +595,7 @@ __device__ __forceinline__ double2* partial_at(float* stats, int groups) { retur
 // other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors, forward: 16.3 us
 // against 16.4 for 512 images of 32x32x32 bf16).  16 vectors leave three workgroups a CU (up to 168 registers); 4 vectors
 // stay within 128, so 1024 threads fit.
-// Bound by HBM: 1024 images of 64x64x32 bf16 with SiLU, four parts each, 98 us for 537 MB = 5.5 TB/s, and 2 us for the launch
+// Bound by HBM: 1024 images of 64x64x32 bf16 with SiLU, four parts each, 103 us for 537 MB = 5.2 TB/s, and 2 us for the launch
 // that empties the words; 512 of 32x32x32 with ReLU and dropout 10 % 14.3 us for 67 MB = 4.7 TB/s (the mask's words are
 // worked out while the loads are in flight).  One image of 64x64x32: 8 us, of which a launch is 2.8 and the rest one
 // memory latency after the other.
@@ -1148,8 +1150,12 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
 // group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
 // linear in it.
 // 16 vectors of x and of dy take 128 registers, all of it up to 256: two workgroups a CU.  Those load together, compute
-// together and store together, so the time is near the sum of both: 64 images of 128x128x32 bf16 with SiLU 51 us for 201 MB
-// (32 of memory at 6.2 TB/s; about 4700 instructions a wave, 27 us), 512 of 32x32x32 with ReLU and dropout 20 for 101 MB.
+// together and store together, so the time is near the sum of both: 64 images of 128x128x32 bf16 with SiLU 45 us for 201 MB
+// (32 of memory at 6.2 TB/s), 512 of 32x32x32 with ReLU and dropout 20 for 101 MB (16).
+// SPLIT: the second pass takes dz as the first one had it, in fp32: its upper halves are where dy was, its lower ones in LDS
+// (64 KB; each thread its own, nothing to wait for).  Working the slope out again instead took 51 us, and for 1024 images of
+// 64x64x32 with GELU 255 where it is 185 now; the bits are the same.  Where a bf16 vector has eight pieces there is no LDS to
+// spare beside the sums of two workgroups, and with 4 vectors a thread nothing to gain.
 // What did not help there: 8 vectors a thread and three workgroups, a staggered start, workgroups that stay and prefetch
 // the next part (their polls and stores queue behind the prefetch: 83 us against 62), loads of x and dy in turn.
 template <typename T, int NS, int I, bool PARTS, int ACT>
