@@ -11,8 +11,23 @@ int launch_gn_fwd_bf16(const NormArgs& a, const Slab* sl, hipStream_t s);
 int launch_gn_bwd_f32(const NormArgs& a, const Slab* sl, hipStream_t s);
 int launch_gn_bwd_bf16(const NormArgs& a, const Slab* sl, hipStream_t s);
 
-// One wave joins the tiles and pieces of a group.  Piece k of an image's tile covers channels k*q .. k*q + q - 1.
-__global__ __launch_bounds__(64) void gn_join_kernel(const NormArgs a) {
+// The sum over a workgroup, the same for all its threads; `shared` holds one value per wave.
+template <typename F> __device__ __forceinline__ F block_total(F v, F* shared) {
+  v = wave_total(v);
+  if (blockDim.x == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = shared[0];
+  for (unsigned w = 1; w < blockDim.x >> 6; ++w) v += shared[w];
+  return v;
+}
+// Joins the tiles and pieces of a group.  Piece k of an image's tile covers channels k*q .. k*q + q - 1.  One wave, or 1024
+// threads where there are many: a wave takes a memory latency for every 64 (22 images of 75x41x617 fp32 in one group, 60,000
+// pieces each, 576 us forward with one wave, 145 so; 9 of 64x64x1024 backward, channels along the threads, 626 and 152).
+constexpr int kJoinThreads = 1024;
+__global__ __launch_bounds__(kJoinThreads) void gn_join_kernel(const NormArgs a) {
+  __shared__ double shared[kJoinThreads / 64];
   const NormGeom& g = a.g;
   const int b = blockIdx.x / g.G, gi = blockIdx.x - b * g.G;
   const int ppg = g.cg / g.q, per_image = g.nv * g.n_slots;
@@ -20,35 +35,37 @@ __global__ __launch_bounds__(64) void gn_join_kernel(const NormArgs a) {
   const float4* part = (const float4*)a.part + (int64_t)b * g.tiles * per_image + gi * ppg;
   const double n_total = (double)g.P * g.cg;
   double s = 0.0, m2 = 0.0;
-  for (int k = threadIdx.x; k < items; k += 64) {
+  for (int k = threadIdx.x; k < items; k += blockDim.x) {
     const int t = k / ppg;
     const float4 p = part[(int64_t)t * per_image + (k - t * ppg)];
     s += (double)p.w * ((double)p.x + (double)p.y);
   }
-  const double mean = wave_total(s) / n_total;
-  for (int k = threadIdx.x; k < items; k += 64) {
+  const double mean = block_total(s, shared) / n_total;
+  for (int k = threadIdx.x; k < items; k += blockDim.x) {
     const int t = k / ppg;
     const float4 p = part[(int64_t)t * per_image + (k - t * ppg)];
     const double d = (double)p.x + (double)p.y - mean;
     m2 += (double)p.z + (double)p.w * (d * d - (double)p.y * (double)p.y);
   }
-  double var = wave_total(m2) / n_total;
+  double var = block_total(m2, shared) / n_total;
   var = var < 0.0 ? 0.0 : var;                                   // a NaN stays
   if (threadIdx.x == 0) {
     a.mean[blockIdx.x] = (float)mean;
     a.rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)a.eps));
   }
 }
-// One wave per (image, group): the image's sums of each channel, and the group's two means.
-__global__ __launch_bounds__(64) void gn_bwd_join_kernel(const NormArgs a, int padded) {
+// One workgroup per (image, group): the image's sums of each channel, and the group's two means.
+__global__ __launch_bounds__(kJoinThreads) void gn_bwd_join_kernel(const NormArgs a, int padded) {
+  __shared__ float shared[kJoinThreads / 64];
   const NormGeom& g = a.g;
   const int b = blockIdx.x / g.G, gi = blockIdx.x - b * g.G;
   float m1 = 0.f, m2 = 0.f;
-  for (int k = threadIdx.x; k < g.cg; k += 64) {
+  for (int k = threadIdx.x; k < g.cg; k += blockDim.x) {
     const int c = gi * g.cg + k;
     const float2* part = a.part + (int64_t)b * g.tiles * padded + c;
     float2 s = make_float2(0.f, 0.f);
-    for (int t = 0; t < g.tiles; ++t) {
+#pragma unroll 8
+    for (int t = 0; t < g.tiles; ++t) {                          // eight loads under way, one order of the sums
       const float2 p = part[(int64_t)t * padded];
       s.x += p.x;
       s.y += p.y;
@@ -58,8 +75,8 @@ __global__ __launch_bounds__(64) void gn_bwd_join_kernel(const NormArgs a, int p
     m1 = fmaf(gamma, s.x, m1);
     m2 = fmaf(gamma, s.y, m2);
   }
-  m1 = wave_total(m1);
-  m2 = wave_total(m2);
+  m1 = block_total(m1, shared);
+  m2 = block_total(m2, shared);
   const float n = (float)g.P * (float)g.cg;
   if (threadIdx.x == 0) a.moments[blockIdx.x] = make_float2(m1 / n, m2 / n);
 }
@@ -105,9 +122,12 @@ void launch_gn_empty(uint64_t* words, int64_t n, hipStream_t s) {
   const int64_t blocks = (n + 255) / 256;
   hipLaunchKernelGGL(gn_empty_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s, words, n);
 }
-void launch_gn_join(const NormArgs& a, hipStream_t s) { hipLaunchKernelGGL(gn_join_kernel, dim3(a.g.B * a.g.G), dim3(64), 0, s, a); }
+void launch_gn_join(const NormArgs& a, hipStream_t s) {
+  const bool many = (int64_t)a.g.tiles * (a.g.cg / a.g.q) > 512;
+  hipLaunchKernelGGL(gn_join_kernel, dim3(a.g.B * a.g.G), dim3(many ? kJoinThreads : 64), 0, s, a);
+}
 void launch_gn_bwd_join(const NormArgs& a, int padded, hipStream_t s) {
-  hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.g.B * a.g.G), dim3(64), 0, s, a, padded);
+  hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.g.B * a.g.G), dim3(a.g.cg > 64 ? kJoinThreads : 64), 0, s, a, padded);
 }
 void launch_gn_param_grads(const NormArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(gn_param_grads_kernel, dim3((a.g.C + 7) / 8), dim3(1024), 0, s, a);
@@ -241,10 +261,10 @@ static int check_range(const NormGeom& g, const char* what) {
                  (int64_t)g.B * g.tiles * g.chunks < (1ll << 31), std::string(what) + ": tensor too large");
   return MI_OK;
 }
-// A launch holds less than 2^32 threads (one wave per image and group in the joins).
+// A launch holds less than 2^32 threads.
 static int check_threads(const NormGeom& g, const Slab* s, const char* what) {
   const int64_t threads = s ? (int64_t)s->img_blocks * s->parts * s->chunks * s->threads
-                            : std::max((int64_t)g.B * g.tiles * g.chunks * kThreads, (int64_t)g.B * g.G * 64);
+                            : std::max((int64_t)g.B * g.tiles * g.chunks * kThreads, (int64_t)g.B * g.G * kJoinThreads);
   MI_REQUIRE(threads < (1ll << 32), std::string(what) + ": tensor too large");
   return MI_OK;
 }
