@@ -31,7 +31,7 @@ inline FastDiv make_fastdiv(uint32_t d) {
   f.d = d;
   return f;
 }
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
+__host__ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
   return (uint32_t)(((uint64_t)n * f.mul) >> f.shift);
 }
 

@@ -1,5 +1,5 @@
-// Group norm: the kernels that do not depend on the stored type, how the work is divided, and the launches by type
-// (norm_f32.hip, norm_bf16.hip; the kernels themselves are in norm_impl.h).
+// Group norm: the kernels that do not depend on the stored type, and the launches by type
+// (norm_f32.hip, norm_bf16.hip; the kernels themselves are in norm_impl.h, the division in norm_division.h).
 #include "norm_impl.h"
 
 #include <algorithm>
@@ -134,111 +134,6 @@ void launch_gn_param_grads(const NormArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- host
-static int gcd_int(int a, int b) {
-  while (b) { const int t = a % b; a = b; b = t; }
-  return a;
-}
-static NormGeom norm_geom(int B, int H, int W, int C, int G, int dtype) {
-  NormGeom g{};
-  const int N = dtype == MI_BF16 ? 8 : 4;
-  g.B = B; g.P = H * W; g.C = C; g.G = G; g.cg = C / G;
-  g.nv = pad_ch(C) / N;
-  while (g.lanes = 1 << g.log_lanes, g.lanes < g.nv && g.lanes < 64) ++g.log_lanes;
-  g.chunks = (g.nv + g.lanes - 1) / g.lanes;
-  g.rows = kThreads / g.lanes;
-  g.tiles = (g.P + g.rows * kI - 1) / (g.rows * kI);
-  g.q = gcd_int(g.cg, N);
-  if (g.q != N && !(N == 8 && g.q == 4)) g.q = 1;                // the kernels come for 1, 2 (bf16) and N pieces per vector
-  g.n_slots = N / g.q;
-  g.d_tiles = make_fastdiv(g.tiles);
-  g.d_chunks = make_fastdiv(g.chunks);
-  g.d_cg = make_fastdiv(g.cg);
-  return g;
-}
-static int pow2_ceil(int64_t v) {
-  int p = 1;
-  while (p < v) p <<= 1;
-  return p;
-}
-// How the slab kernels divide the work, or false where they do not apply.
-// Up to 64 parts, which run at the same time on a fraction of the card.  Without parts, by the general kernels: 16 images of 128x128x64
-// bf16 20 us forward and 75 backward, with them 14 and 25; 2 of 256x256x32 12.7 and 50 against 13.6 and 20.
-constexpr int kMaxParts = 64;
-constexpr int kPolls = 4096;                 // about 1 us each
-// The division with `iters` vectors a thread of chunks of cv vectors, up to `most` threads for an image, `most_nb` for several.
-static bool divide_slab(const NormGeom& g, int64_t cv, int iters, int most, int most_nb, Slab* out) {
-  Slab s{};
-  s.iters = iters;
-  s.cv = (int)cv;
-  s.lanes = pow2_ceil(cv);
-  while ((1 << s.log_lanes) < s.lanes) ++s.log_lanes;
-  s.chunks = (int)((g.nv + cv - 1) / cv);
-  const int64_t vectors = (int64_t)g.P * s.lanes;
-  s.tpi = vectors < iters * most ? pow2_ceil((vectors + iters - 1) / iters) : most;
-  if (s.tpi < s.lanes) s.tpi = s.lanes;
-  while ((1 << s.log_tpi) < s.tpi) ++s.log_tpi;
-  s.rows = s.tpi / s.lanes;
-  const int64_t parts = (g.P + (int64_t)s.rows * iters - 1) / ((int64_t)s.rows * iters);
-  if (parts > kMaxParts) return false;
-  s.parts = (int)parts;
-  s.nb = 1;
-  if (s.parts == 1)
-    while (s.nb * s.tpi < most_nb && s.nb < g.B) s.nb *= 2;
-  s.img_blocks = (g.B + s.nb - 1) / s.nb;
-  s.threads = s.nb * s.tpi < 64 ? 64 : s.nb * s.tpi;
-  const int ppg = g.cg / g.q;
-  s.merge = g.n_slots == 1 && (ppg & (ppg - 1)) == 0 ? ppg : 1;
-  s.left = ppg / s.merge;
-  s.polls = kPolls;
-  s.d_chunks = make_fastdiv(s.chunks);
-  s.d_parts = make_fastdiv(s.parts);
-  *out = s;
-  return true;
-}
-static bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
-  const int unit = g.cg / gcd_int(g.cg, N) < g.nv ? g.cg / gcd_int(g.cg, N) : g.nv;   // vectors after which a group ends with a vector
-  if (unit > 64) return false;
-  const int64_t most = 16 * kSlabThreads, few = 4 * kSlabThreads;
-  const bool small = (int64_t)g.B * g.P * g.nv < 256 * most;     // not enough to give every CU a full workgroup
-  int64_t cv = g.nv <= 64 ? g.nv : unit * (64 / unit);
-  // Fewer workgroups than CUs: narrower chunks, down to one line of 128 bytes per pixel, or to 64 bytes where an image's
-  // chunk then has a workgroup of its own.  Measured, forward / backward: 8 images of 4x4x1024 fp32 4.0 / 7.0 us with whole
-  // pixels, 3.7 / 6.5 so; 32 of 16x16x64 bf16 6.0 / 11.3 with 128 bytes, 4.3 / 8.1 with 64 (with 32: 5.0 / 8.7); but
-  // 16 of 128x128x64 bf16, which have parts, 14.1 / 24.3 with 128 bytes and 18.8 / 38 with 64.
-  // Backward, an image of more than 64 parts is cut into narrower chunks whatever their number: one of 256x256x512 fp32 616 us
-  // by the general kernels, 151 in chunks of 64 bytes, 16 of 256x256x64 bf16 225 and 124; forward 120 and 146, 88 and 106.
-  for (;;) {
-    const int64_t lanes = pow2_ceil(cv), size = g.P * lanes, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
-    int64_t half = cv / 2 / unit * unit;
-    if (2 * pow2_ceil(half) < lanes) half = lanes / 2 / unit * unit;
-    const bool cut = backward && size > kMaxParts * most;
-    const int64_t least = cut || g.P * (int64_t)pow2_ceil(half) <= most ? 4 : 8;
-    if (pow2_ceil(half) < least || (!cut && (wgs >= 256 || size <= 256))) break;
-    cv = half;
-  }
-  // And below that, down to a lane, where it spares an image of a tensor of at most 256 KB its parts, whose words take a
-  // launch to empty: one image of 64x64x32 bf16 8.0 us forward and 11.1 backward on the device, with parts 8.0 and 11.7, and
-  // 3 us less on the host.  Larger tensors lose more by the lines read in pieces: one image of 64x64x64 11 and 23 us, with
-  // parts 7.7 and 11.5; 8 of 64x64x32 10.8 and 19.7, with parts 8.4 and 13.3.
-  if ((int64_t)g.B * g.P * g.nv <= 4 * most && g.P * (int64_t)pow2_ceil(cv) > most) {
-    int64_t narrow = cv;
-    while (narrow >= unit && g.P * (int64_t)pow2_ceil(narrow) > most) narrow = narrow / 2 / unit * unit;
-    if (narrow >= unit) cv = narrow;
-  }
-  const int64_t vectors = (int64_t)g.P * pow2_ceil(cv);
-  // 16 vectors a thread, as many as its registers hold, where that leaves every CU a workgroup; else 4, and a fourth of the
-  // time.  An image of up to 4096 vectors then has up to 1024 threads, to be spared parts; backward, all images of a chunk
-  // share these threads if they can, and no launch has to join the parameter gradients.  Measured, forward / backward:
-  // 512 images of 4x4x256 bf16 4.5 / 10 us, with 16 vectors 6.2 / 15.2; 64 of 8x8x512 fp32 5.7 / 9.4 with 1024 threads,
-  // 6.6 / 11.3 with 16 vectors and 256; 8 of 4x4x1024 fp32 backward 4.7 and 6.5.
-  const bool alone = backward && g.B <= kSlabThreads && pow2_ceil(g.B) * vectors <= most;
-  int iters = small ? 4 : 16;
-  if (vectors <= pow2_ceil(cv)) iters = 1;
-  else if (alone && pow2_ceil(g.B) * vectors <= few) iters = 4;
-  const int threads = small && vectors <= most ? kWideThreads : kSlabThreads;
-  return divide_slab(g, cv, iters, iters == 4 ? threads : kSlabThreads, alone && iters == 4 ? threads : kSlabThreads, out) ||
-         divide_slab(g, cv, 16, kSlabThreads, kSlabThreads, out);
-}
 static size_t slab_rows(const Slab& s) { return (size_t)s.img_blocks * s.parts; }   // rows of channel sums
 static size_t fwd_part_bytes(const NormGeom& g) { return (size_t)g.B * g.tiles * g.nv * g.n_slots * sizeof(float4); }
 static size_t bwd_part_bytes(const NormGeom& g, int dtype) {

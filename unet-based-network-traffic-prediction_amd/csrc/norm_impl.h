@@ -25,23 +25,11 @@
 // Sums have a fixed order: results repeat bit for bit.
 #pragma once
 #include "drop.h"
+#include "norm_division.h"
 
 #include <type_traits>
 
 namespace mi {
-
-constexpr int kThreads = 256, kWaves = kThreads / 64, kI = 8;
-
-struct NormGeom {
-  int B, P, C, G, cg;
-  int nv;                      // vectors per pixel
-  int lanes, log_lanes;        // lanes per pixel: power of two, at most 64
-  int chunks;                  // ranges of `lanes` vectors that make up a pixel
-  int rows;                    // pixels read at a time = kThreads / lanes
-  int tiles;                   // per image
-  int q, n_slots;              // channels that are summed together (a vector, 4 of a bf16 vector, or 1: must divide cg), pieces per vector
-  FastDiv d_tiles, d_chunks, d_cg;
-};
 
 struct NormArgs {
   NormGeom g;
@@ -282,21 +270,6 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const NormArgs a) {
 //
 // A workgroup owns `nb` images x cv vectors.  Its threads are (image, row, lane): lanes lie along the channels, tpi
 // threads share an image.  A group's sum goes over the rows and lanes of a wave by shuffles and over waves through LDS.
-constexpr int kSlabThreads = 256, kWideThreads = 1024;
-struct Slab {
-  int cv;                      // vectors per pixel of a chunk: whole groups
-  int lanes, log_lanes;        // power of two >= cv, at most 64
-  int chunks;
-  int tpi, log_tpi;            // threads per image, a power of two >= lanes
-  int nb, img_blocks;          // images per workgroup, workgroups along the images
-  int rows;                    // tpi / lanes
-  int parts;                   // workgroups that share an image (then nb = 1, tpi = kSlabThreads)
-  int merge;                   // lanes of a group that shuffles can sum (a power of two), ...
-  int left;                    // ... and what then remains: pieces per group / merge
-  int threads, iters;          // nb * tpi, pixels per thread
-  int polls;                   // how often a part is looked for before its sums are formed here instead
-  FastDiv d_chunks, d_parts;
-};
 struct SlabThread {
   int tin, slot, lane, row;    // thread of its image, image of the workgroup, vector of the chunk, row of pixels
   int b, v, part, chunk;       // image, vector
@@ -354,8 +327,12 @@ template <int I> __device__ __forceinline__ void zero_missing(const SlabPixels& 
 template <int WHICH = -1> __device__ __forceinline__ void pin(u32x4_t& v, float after) {
   asm volatile("; %1" : "+v"(v) : "n"(WHICH), "v"(after));
 }
+__device__ __forceinline__ int opaque(int v) {                   // a value whose uses are not prepared in advance
+  asm volatile("" : "+v"(v));
+  return v;
+}
 // K sums over each group of each image: in, a thread's K x NS partial sums (of its vector's pieces); out, the sums of the
-// groups that its pieces belong to.  `shared`: as much as slab_shared says; free to use again after a barrier.
+// groups that its pieces belong to.  `shared`: as much as slab_sum_floats says; free to use again after a barrier.
 template <int NS, int K>
 __device__ __forceinline__ void slab_sum(float (&v)[K][NS], const NormGeom& g, const Slab& s, const SlabThread& t, float* shared) {
   for (int o = min(64, s.tpi) >> 1; o >= s.lanes; o >>= 1) {
@@ -392,11 +369,7 @@ __device__ __forceinline__ void slab_sum(float (&v)[K][NS], const NormGeom& g, c
   }
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    int first = t.lane * NS + j;
-    if (s.left > 1) {                                            // the first piece of this piece's group, within the chunk
-      const int c = min((t.chunk * s.cv + t.lane) * (NS * g.q) + j * g.q, g.C - 1);
-      first = ((int)fdiv((uint32_t)c, g.d_cg) * g.cg) / g.q - t.chunk * s.cv * NS;
-    }
+    const int first = slab_first_piece(g, s, NS, t.chunk, t.lane, j);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float sum = 0.f;
@@ -473,7 +446,7 @@ __device__ __forceinline__ void slab_moments(const V& v, const SlabPixels& px, c
     q[j] = fmaf(-m[j], sum[0][j], sum[1][j]);
     far = far || !(4.f * q[j] >= sum[1][j]);
   }
-  if (__syncthreads_or(far && t.live)) {
+  if (__syncthreads_or(far && t.live && t.v * N < g.C)) {        // vectors of padding may hold anything
     float dev[2][NS] = {};
 #pragma unroll V::kUnroll
     for (int i = 0; i < I; ++i) {
@@ -582,15 +555,6 @@ __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeo
   __syncthreads();
   return result;
 }
-// Where the groups' results lie in LDS: behind the 2 * NS sums of slab_sum (parts > 1: one image, all its threads).
-template <int NS> __device__ __forceinline__ int slab_stats_at(const Slab& s) {
-  return s.tpi <= 64 && s.left == 1 ? 0 : ((s.threads + 63) >> 6) * s.lanes * 2 * NS;
-}
-// Behind them, the number of a missing part, and the sums of the waves.
-constexpr int kPartialFloats = kSlabThreads * 4;
-__device__ __forceinline__ int* missing_at(float* stats, int groups) { return (int*)(stats + 2 * groups); }
-__device__ __forceinline__ double2* partial_at(float* stats, int groups) { return (double2*)(stats + ((2 * groups + 5) & ~3)); }
-
 // 256 threads with up to 16 vectors each: what a thread does once -- its place, its channels' parameters, the sums over
 // other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors, forward: 16.3 us
 // against 16.4 for 512 images of 32x32x32 bf16).  16 vectors leave three workgroups a CU (up to 168 registers); 4 vectors
@@ -635,14 +599,15 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
       rstd[j] = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);    // a NaN stays
     }
   } else {
-    float* stats = shared + slab_stats_at<NS>(s);                // (mean, rstd) of each group of the chunk, then one int
-    const int g0 = t.chunk * s.cv * N / g.cg, groups = min(s.cv * N / g.cg, g.G - g0);
+    float* stats = shared + slab_stats_at(s, NS);                // (mean, rstd) of each group of the chunk, then one int
+    const int g0 = slab_first_group(g, s, N, t.chunk), groups = slab_groups(g, s, N, t.chunk);
     uint64_t* words = a.words + 2 * ((int64_t)t.b * s.parts * g.G + g0);
     auto publish = [&](int part) {
       if (t.row != 0 || !t.live) return;
+      const int c1 = opaque(c0);
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
-        const int c = c0 + j * Q, gi = (int)fdiv((uint32_t)min(c, g.C - 1), g.d_cg);
+        const int c = c1 + j * Q, gi = (int)fdiv((uint32_t)min(c, g.C - 1), g.d_cg);
         if (c != gi * g.cg) continue;                            // not a group's first piece
         uint64_t* w = words + 2 * ((int64_t)part * g.G + gi - g0);
         put_word(w, (uint64_t)__double_as_longlong((double)mean[j] + (double)e[j]));
@@ -652,7 +617,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
     publish(t.part);
     for (;;) {
       // deviations from part 0's mean: those of the means themselves, so nothing cancels that 64 bits would miss
-      const int part = slab_collect<2>(words, g, s, groups, missing_at(stats, groups), partial_at(stats, groups),
+      const int part = slab_collect<2>(words, g, s, groups, (int*)(stats + slab_missing_at(groups)), (double2*)(stats + slab_partial_at(groups)),
         [&](int p, uint64_t w0, uint64_t w1, uint64_t first, double& s0, double& s1) {
           const double n = (double)min(g.P - p * s.rows * I, s.rows * I) * g.cg;
           const double d = __longlong_as_double((long long)w0) - __longlong_as_double((long long)first);
@@ -670,9 +635,10 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
       publish(part);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // the next look finds it
     }
+    const int c1 = opaque(c0);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int gi = (int)fdiv((uint32_t)min(c0 + j * Q, g.C - 1), g.d_cg) - g0;
+      const int gi = slab_group_of(g, s, N, t.chunk, c1 + j * Q);
       mean[j] = stats[2 * gi];
       rstd[j] = stats[2 * gi + 1];
     }
@@ -892,10 +858,6 @@ template <int NS, int N> __device__ __forceinline__ void slab_scale(const float*
 #pragma unroll
   for (int j = 0; j < N; ++j) scaled[j] *= rstd[j * NS / N];
 }
-__device__ __forceinline__ int opaque(int v) {                   // a value whose uses are not prepared in advance
-  asm volatile("" : "+v"(v));
-  return v;
-}
 // Publishes a part's two sums of each group.
 template <int NS, int N>
 __device__ __forceinline__ void publish_bwd(const NormArgs& a, const SlabThread& t, int part, const float (&sum)[2][NS]) {
@@ -1071,12 +1033,12 @@ __device__ __forceinline__ void bwd_means(const NormArgs& a, const Slab& s, cons
       sum[1][j] *= inv;
     }
   } else {
-    const int g0 = t.chunk * s.cv * N / g.cg, groups = min(s.cv * N / g.cg, g.G - g0);
+    const int g0 = slab_first_group(g, s, N, t.chunk), groups = slab_groups(g, s, N, t.chunk);
     const uint64_t* words = a.words + ((int64_t)t.b * s.parts * g.G + g0);
-    float* stats = shared + slab_stats_at<NS>(s);
+    float* stats = shared + slab_stats_at(s, NS);
     __syncthreads();
     for (;;) {
-      const int part = slab_collect<1>(words, g, s, groups, missing_at(stats, groups), partial_at(stats, groups),
+      const int part = slab_collect<1>(words, g, s, groups, (int*)(stats + slab_missing_at(groups)), (double2*)(stats + slab_partial_at(groups)),
         [&](int, uint64_t w, uint64_t, uint64_t, double& s0, double& s1) {
           s0 += (double)__uint_as_float((uint32_t)w);
           s1 += (double)__uint_as_float((uint32_t)(w >> 32));
@@ -1089,9 +1051,10 @@ __device__ __forceinline__ void bwd_means(const NormArgs& a, const Slab& s, cons
       if (__builtin_expect(part < 0, 1)) break;
       bwd_other_part<T, NS, I, ACT>(a, s, t, part, shared);
     }
+    const int c0 = opaque(t.v * N);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int gi = (int)fdiv((uint32_t)min(t.v * N + j * (N / NS), g.C - 1), g.d_cg) - g0;
+      const int gi = slab_group_of(g, s, N, t.chunk, c0 + j * (N / NS));
       sum[0][j] = stats[2 * gi];
       sum[1][j] = stats[2 * gi + 1];
     }
@@ -1209,21 +1172,12 @@ void launch_gn_join(const NormArgs& a, hipStream_t s);
 void launch_gn_bwd_join(const NormArgs& a, int padded, hipStream_t s);
 void launch_gn_param_grads(const NormArgs& a, hipStream_t s);
 
-inline unsigned slab_grid(const Slab& s) { return (unsigned)(s.img_blocks * s.parts * s.chunks); }
-// 64-bit words that the parts exchange
-inline int64_t slab_words(const NormGeom& g, const Slab& s) { return 2 * (int64_t)g.B * s.parts * g.G; }
-// LDS floats of slab_sum with K sums of NS pieces
-inline int slab_sum_floats(const Slab& s, int sums) {
-  if (s.tpi <= 64 && s.left == 1) return 0;
-  return (s.tpi > 64 ? s.threads >> 6 : s.threads >> s.log_tpi) * s.lanes * sums;
-}
 // bf16 vectors of two pieces (groups of 4, 12, 20, ... channels); N / 4 is 1 in fp32, where there is no such kernel
 template <typename T> bool two_pieces(const NormGeom& g) { return ActVec<T>::N == 8 && g.n_slots == 2; }
 template <typename T, int NS>
 void launch_fwd_slab(const NormArgs& a, const Slab& sl, hipStream_t s) {
   const dim3 grid(slab_grid(sl)), block((unsigned)sl.threads);
-  // the sums, and with several parts (mean, rstd) of each group of the chunk and a number
-  const int floats = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 + kPartialFloats : 0);
+  const int floats = slab_fwd_floats(a.g, sl, NS, ActVec<T>::N);
   const unsigned lds = (unsigned)(floats * sizeof(float));
   if (sl.parts > 1) launch_gn_empty(a.words, slab_words(a.g, sl), s);
 #define GN_SLAB(I, PARTS) hipLaunchKernelGGL((gn_fwd_slab_kernel<T, NS, I, PARTS>), grid, block, lds, s, a, sl)
@@ -1266,11 +1220,7 @@ void launch_bwd_slab_act(const NormArgs& a, const Slab& sl, dim3 grid, dim3 bloc
 template <typename T, int NS>
 void launch_bwd_slab(const NormArgs& a, const Slab& sl, hipStream_t s) {
   const dim3 grid(slab_grid(sl)), block((unsigned)sl.threads);
-  const int sums = slab_sum_floats(sl, 2 * NS) + (sl.parts > 1 ? 2 * (sl.cv * ActVec<T>::N / a.g.cg + 1) + 2 + kPartialFloats : 0);
-  const int channels = a.dgamma || a.dbeta ? (sl.threads >> 6) * sl.lanes * 2 * ActVec<T>::N : 0;
-  const int thresholds = a.act == MI_ACT_RELU ? (sl.threads >> sl.log_tpi) * sl.lanes * ActVec<T>::N : 0;
-  int floats = sums > channels ? sums : channels;
-  if (thresholds > floats) floats = thresholds;
+  const int floats = slab_bwd_floats(a.g, sl, NS, ActVec<T>::N, a.dgamma || a.dbeta, a.act == MI_ACT_RELU);
   const unsigned lds = (unsigned)(floats * sizeof(float));
   if (sl.parts > 1) launch_gn_empty(a.words, slab_words(a.g, sl) / 2, s);
 #define GN_SLAB(A) launch_bwd_slab_act<T, NS, A>(a, sl, grid, block, lds, s)
