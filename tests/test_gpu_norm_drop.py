@@ -661,3 +661,40 @@ def test_refusals_on_the_gpu(ua):
     assert dx.shape == (0, 4, 4, 48) and (dw == 0).all() and (db == 0).all()
     assert ops.dropout_fwd(empty, 40, drop).shape == (0, 4, 4, 48)
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- values whose squares pass fp32's range
+LARGE = [(2, 8, 8, 64, 8), (5, 8, 8, 64, 16), (3, 9, 8, 72, 24), (2, 1, 1, 1024, 4), (1, 64, 64, 32, 8), (12, 90, 80, 32, 4), (9, 100, 96, 40, 8),
+         (2, 70, 67, 36, 12), (1, 256, 255, 66, 6), (3, 256, 250, 64, 4)]      # one workgroup an image, several, the general kernels
+
+
+def grouped(scales, B, C, G):
+    """(B, 1, 1, C): a scale for each group, the next image's one further on."""
+    s = torch.tensor([[scales[(b + g) % len(scales)] for g in range(G)] for b in range(B)], dtype=torch.float64)
+    return N._per_channel(s, C // G)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", LARGE)
+def test_norm_of_large_values(ua, monkeypatch, dtype, shape):
+    """Finite groups whose sum of squares, or whose sum, fp32 does not hold, beside ordinary ones."""
+    B, H, W, C, G = shape
+    ops = ua.ops
+    scale, shift = grouped([1.0, 1e18, 1e25, 2e36], B, C, G), grouped([0.0, 0.0, 1e27, 0.0, 1.0, 1e20], B, C, G)
+    x = ((rnd(1, B, H, W, C) + rnd(2, C)) * scale + shift).to(dtype)
+    assert torch.isfinite(x).all()
+    gamma, beta = rnd(3, C, scale=0.3, shift=1.0), rnd(4, C, scale=0.3)
+    y, mean, rstd = ops.group_norm_act_fwd(place(x, dtype), C, G, gamma.cuda(), beta.cuda(), act="silu")
+    x6, g6, b6 = x.double(), gamma.double(), beta.double()
+    oy, om, orr, z = N.group_norm_act_fwd(x6, G, g6, b6, "silu", float(torch.tensor(1e-5)))
+    dm, dr, _ = stats_bounds(x6, om, orr, G)
+    within(mean, om, dm + 1e-37, "mean")
+    within(rstd, orr, dr, "rstd")
+    within(y[..., :C], oy, fwd_bound(x6, oy, z, om, orr, g6, b6, G, dtype), "y")
+    check_padding(y, C)
+    monkeypatch.setattr(ops, "_POLLS", 0)
+    again = ops.group_norm_act_fwd(place(x, dtype), C, G, gamma.cuda(), beta.cuda(), act="silu")
+    assert all(torch.equal(s, t) for s, t in zip((y, mean, rstd), again))
+    same = torch.full((B, H, W, C), 2.0 ** 100)                   # no deviations at all: z = beta
+    y, mean, rstd = ops.group_norm_act_fwd(place(same, dtype), C, G, None, beta.cuda())
+    assert (mean == 2.0 ** 100).all() and torch.equal(y[..., :C].float().cpu(), beta.to(dtype).float().expand(B, H, W, C))

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kJoinThreads) void gn_join_kernel(const NormArgs a)
     const int t = k / ppg;
     const float4 p = part[(int64_t)t * per_image + (k - t * ppg)];
     const double d = (double)p.x + (double)p.y - mean;
-    m2 += (double)p.z + (double)p.w * (d * d - (double)p.y * (double)p.y);
+    m2 += unmarked(p.z) + (double)p.w * (d * d - (double)p.y * (double)p.y);
   }
   double var = block_total(m2, shared) / n_total;
   var = var < 0.0 ? 0.0 : var;                                   // a NaN stays

@@ -185,47 +185,90 @@ __device__ __forceinline__ void load_groups(const float* p, const NormGeom& g, i
   for (int j = 0; j < N; ++j) out[j] = p[(int64_t)b * g.G + fdiv((uint32_t)min(c0 + j, g.C - 1), g.d_cg)];
 }
 
+__device__ __forceinline__ int opaque(int v) {                   // a value whose uses are not prepared in advance
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// Ends the lifetime of what was derived from v: without it the compiler unpacks the vectors of all of a thread's pixels in
+// advance and keeps them (bf16: twice the registers of the vectors) from one use to the next.  `after` is a result that
+// the use has to wait for; WHICH tells branches of one switch apart, whose common beginnings would otherwise move in front
+// of the switch.
+template <int WHICH = -1> __device__ __forceinline__ void pin(u32x4_t& v, float after) {
+  asm volatile("; %1" : "+v"(v) : "n"(WHICH), "v"(after));
+}
+// Values whose squares pass fp32's range are summed as their 2^-80th part (which costs nothing: what underflows is too small to
+// count among them).  Squared deviations that still pass it are handed on in that scale, with their sign turned.
+constexpr float kTiny = 0x1p-80f;
+__device__ __forceinline__ float unscaled_or_marked(float q) {
+  const float all = q * (1.f / kTiny) * (1.f / kTiny);
+  return all < INFINITY ? all : -q;                              // a NaN stays
+}
+__device__ __forceinline__ double unmarked(float q) { return q < 0.f ? (double)q * -0x1p160 : (double)q; }
 // Forward, statistics of a tile: (m, r / n, q, n) of each piece (q channels of one vector).
 template <typename T, int NS>
 __global__ __launch_bounds__(kThreads) void gn_stats_kernel(const NormArgs a) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   __shared__ float shared[kWaves * 64 * NS];
   const NormGeom& g = a.g;
-  const Tile w = my_tile(g);
-  u32x4_t v[kI];
-  load_tile<T>(w, g, a.x, a.xcs, a.xco, v);
-  float s[NS] = {}, m[NS], r[NS] = {}, q[NS] = {};
-#pragma unroll
-  for (int i = 0; i < kI; ++i) {
-    float f[N];
-    ActVec<T>::unpack(v[i], f);
-#pragma unroll
-    for (int j = 0; j < N; ++j) s[j / Q] += i < w.n ? f[j] : 0.f;
-  }
-  tile_sum<NS>(s, g, shared);
+  Tile w = my_tile(g);
   const float n = (float)w.count * Q;
   const int lane = threadIdx.x & (g.lanes - 1);
+  float m[NS], r[NS], q[NS], scale[NS];
 #pragma unroll
-  for (int j = 0; j < NS; ++j) m[j] = shared[lane * NS + j] / n;
+  for (int j = 0; j < NS; ++j) scale[j] = 1.f;
+  for (bool again = false;; again = true) {                      // mostly once: nothing is kept for a second time
+    u32x4_t v[kI];
+    w.row = opaque(w.row);
+    load_tile<T>(w, g, a.x, a.xcs, a.xco, v);
+    float s[NS];
 #pragma unroll
-  for (int i = 0; i < kI; ++i) {
-    float f[N];
-    ActVec<T>::unpack(v[i], f);
+    for (int j = 0; j < NS; ++j) s[j] = r[j] = q[j] = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float d = i < w.n ? f[j] - m[j / Q] : 0.f;
-      r[j / Q] += d;
-      q[j / Q] = fmaf(d, d, q[j / Q]);
+    for (int i = 0; i < kI; ++i) {
+      float f[N];
+      ActVec<T>::unpack(v[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s[j / Q] = i < w.n ? fmaf(f[j], scale[j / Q], s[j / Q]) : s[j / Q];
     }
-  }
-  tile_sum<NS>(r, g, shared);
+    tile_sum<NS>(s, g, shared);
 #pragma unroll
-  for (int j = 0; j < NS; ++j) r[j] = shared[lane * NS + j];
-  tile_sum<NS>(q, g, shared);
+    for (int j = 0; j < NS; ++j) m[j] = shared[lane * NS + j] / n;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+      float f[N];
+      ActVec<T>::unpack(v[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = i < w.n ? fmaf(f[j], scale[j / Q], -m[j / Q]) : 0.f;
+        r[j / Q] += d;
+        q[j / Q] = fmaf(d, d, q[j / Q]);
+      }
+    }
+    tile_sum<NS>(r, g, shared);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) r[j] = shared[lane * NS + j];
+    tile_sum<NS>(q, g, shared);
+    bool big = false;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      q[j] = shared[lane * NS + j];
+      big = big || !(q[j] < INFINITY);
+    }
+    if (again || !__syncthreads_or(big && w.live && w.v * N < g.C)) break;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) scale[j] = q[j] < INFINITY ? 1.f : kTiny;      // the others come out the same again
+  }
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    if (scale[j] == 1.f) continue;
+    m[j] *= 1.f / kTiny;
+    r[j] *= 1.f / kTiny;
+    q[j] = unscaled_or_marked(q[j]);
+  }
   if ((int)threadIdx.x < g.lanes && w.live) {
     float4* out = (float4*)a.part + (((int64_t)w.b * g.tiles + w.t) * g.nv + w.v) * NS;
 #pragma unroll
-    for (int j = 0; j < NS; ++j) out[j] = make_float4(m[j], r[j] / n, shared[lane * NS + j], n);
+    for (int j = 0; j < NS; ++j) out[j] = make_float4(m[j], r[j] / n, q[j], n);
   }
 }
 template <typename T, int ACT>
@@ -319,17 +362,6 @@ template <int I> __device__ __forceinline__ void zero_missing(const SlabPixels& 
   if (px.full) return;
 #pragma unroll
   for (int i = 0; i < I; ++i) v[i] = i < px.mine ? v[i] : u32x4_t{0, 0, 0, 0};
-}
-// Ends the lifetime of what was derived from v: without it the compiler unpacks the vectors of all of a thread's pixels in
-// advance and keeps them (bf16: twice the registers of the vectors) from one use to the next.  `after` is a result that
-// the use has to wait for; WHICH tells branches of one switch apart, whose common beginnings would otherwise move in front
-// of the switch.
-template <int WHICH = -1> __device__ __forceinline__ void pin(u32x4_t& v, float after) {
-  asm volatile("; %1" : "+v"(v) : "n"(WHICH), "v"(after));
-}
-__device__ __forceinline__ int opaque(int v) {                   // a value whose uses are not prepared in advance
-  asm volatile("" : "+v"(v));
-  return v;
 }
 // K sums over each group of each image: in, a thread's K x NS partial sums (of its vector's pieces); out, the sums of the
 // groups that its pieces belong to.  `shared`: as much as slab_sum_floats says; free to use again after a barrier.
@@ -428,7 +460,8 @@ __device__ __forceinline__ InMemory<T, I> in_memory(const SlabThread& t, const S
 }
 // Mean (as m + e, m rounded) and squared deviations of the groups over a part.  Sums of x and x^2 first: they do where
 // the deviations are not small against the values, 4 q >= sum x^2 -- what is lost then are two bits.  Groups further from
-// zero take the corrected two-pass form.  Which of the two is decided for each group by its own values.
+// zero take the corrected two-pass form, and so do those whose sum of squares passes fp32's range: their values are scaled
+// first.  Which of them is decided for each group by its own values.
 template <typename T, int NS, int I, typename V>
 __device__ __forceinline__ void slab_moments(const V& v, const SlabPixels& px, const NormGeom& g, const Slab& s, const SlabThread& t,
                                              float* shared, float* m, float* e, float* q) {
@@ -444,9 +477,31 @@ __device__ __forceinline__ void slab_moments(const V& v, const SlabPixels& px, c
     m[j] = sum[0][j] * inv;
     e[j] = 0.f;
     q[j] = fmaf(-m[j], sum[0][j], sum[1][j]);
-    far = far || !(4.f * q[j] >= sum[1][j]);
+    far = far || !(fmaf(4.f, q[j], -sum[1][j]) >= 0.f);          // also where both are infinite
   }
-  if (__syncthreads_or(far && t.live && t.v * N < g.C)) {        // vectors of padding may hold anything
+  const bool real = t.live && t.v * N < g.C;                     // vectors of padding may hold anything
+  if (__syncthreads_or(far && real)) {
+    float scale[NS];
+    bool big = false;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      scale[j] = sum[1][j] < INFINITY ? 1.f : kTiny;
+      big = big || scale[j] != 1.f;
+    }
+    if (__syncthreads_or(big && real)) {
+      float sums[1][NS] = {};
+#pragma unroll V::kUnroll
+      for (int i = 0; i < I; ++i) {
+        float f[N];
+        ActVec<T>::unpack(v(i, m[0]), f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sums[0][j / Q] = fmaf(f[j], scale[j / Q], sums[0][j / Q]);
+      }
+      slab_sum<NS, 1>(sums, g, s, t, shared);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) m[j] = scale[j] == 1.f ? m[j] : sums[0][j] * inv;
+      __syncthreads();
+    }
     float dev[2][NS] = {};
 #pragma unroll V::kUnroll
     for (int i = 0; i < I; ++i) {
@@ -454,7 +509,7 @@ __device__ __forceinline__ void slab_moments(const V& v, const SlabPixels& px, c
       ActVec<T>::unpack(v(i, m[0]), f);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float d = i < px.mine ? f[j] - m[j / Q] : 0.f;
+        const float d = i < px.mine ? fmaf(f[j], scale[j / Q], -m[j / Q]) : 0.f;
         dev[0][j / Q] += d;
         dev[1][j / Q] = fmaf(d, d, dev[1][j / Q]);
       }
@@ -462,9 +517,14 @@ __device__ __forceinline__ void slab_moments(const V& v, const SlabPixels& px, c
     slab_sum<NS, 2>(dev, g, s, t, shared);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      if (4.f * q[j] >= sum[1][j]) continue;
+      if (fmaf(4.f, q[j], -sum[1][j]) >= 0.f) continue;
       e[j] = dev[0][j] * inv;
       q[j] = fmaf(-e[j], dev[0][j], dev[1][j]);
+      q[j] = q[j] < 0.f ? 0.f : q[j];                            // a NaN stays
+      if (scale[j] == 1.f) continue;
+      m[j] *= 1.f / kTiny;
+      e[j] *= 1.f / kTiny;
+      q[j] = unscaled_or_marked(q[j]);
     }
     __syncthreads();
   }
@@ -596,7 +656,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
     for (int j = 0; j < NS; ++j) {
       const float var = q[j] * inv;
       mean[j] += e[j];
-      rstd[j] = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);    // a NaN stays
+      rstd[j] = var < 0.f ? kTiny / sqrtf(-var) : 1.f / sqrtf(var + a.eps);
     }
   } else {
     float* stats = shared + slab_stats_at(s, NS);                // (mean, rstd) of each group of the chunk, then one int
@@ -611,7 +671,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
         if (c != gi * g.cg) continue;                            // not a group's first piece
         uint64_t* w = words + 2 * ((int64_t)part * g.G + gi - g0);
         put_word(w, (uint64_t)__double_as_longlong((double)mean[j] + (double)e[j]));
-        put_word(w + 1, (uint64_t)__double_as_longlong((double)q[j]));
+        put_word(w + 1, (uint64_t)__double_as_longlong(unmarked(q[j])));
       }
     };
     publish(t.part);
