@@ -698,3 +698,16 @@ def test_norm_of_large_values(ua, monkeypatch, dtype, shape):
     same = torch.full((B, H, W, C), 2.0 ** 100)                   # no deviations at all: z = beta
     y, mean, rstd = ops.group_norm_act_fwd(place(same, dtype), C, G, None, beta.cuda())
     assert (mean == 2.0 ** 100).all() and torch.equal(y[..., :C].float().cpu(), beta.to(dtype).float().expand(B, H, W, C))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 8, 8, 64, 8), (3, 1, 2, 64, 64), (2, 128, 128, 40, 5), (1, 256, 255, 66, 3)])
+def test_relu_gate_without_deviation(ua, dtype, shape):
+    """rstd = 0 (an infinite eps, or what a caller handed in): z = beta, so the gate is beta's sign."""
+    B, H, W, C, G = shape
+    x, dy, beta = rnd(1, B, H, W, C).to(dtype), torch.ones(B, H, W, C), rnd(2, C)
+    beta[::7] = 0
+    dx, dw, db = ua.ops.group_norm_act_bwd(place(x, dtype), place(dy, dtype), torch.zeros(B, G).cuda(), torch.zeros(B, G).cuda(), C, G,
+                                           rnd(3, C).cuda(), beta.cuda(), act="relu")
+    assert torch.equal(db.cpu(), (beta > 0).float() * (B * H * W))            # counts below 2^24: exact
+    assert (dw == 0).all() and (dx == 0).all()

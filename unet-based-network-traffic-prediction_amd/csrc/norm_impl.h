@@ -869,7 +869,7 @@ __device__ __forceinline__ float relu_threshold(float mean, float rstd, float ga
   const float f = (float)tau;
   const float below = f > 0.f ? __uint_as_float(__float_as_uint(f) - 1) : __uint_as_float(f < 0.f ? __float_as_uint(f) + 1 : 0x80000001u);
   const float t = (double)f > tau ? below : f;                   // f itself where tau is an fp32 value, infinite or NaN
-  return gamma == 0.f ? (beta > 0.f ? -INFINITY : INFINITY) : t;
+  return d == 0.0 ? (beta > 0.f ? -INFINITY : INFINITY) : t;     // z = beta
 }
 __device__ __forceinline__ bool relu_gate(float x, float gamma, float threshold) {
   return __uint_as_float(__builtin_amdgcn_bitop3_b32(__float_as_uint(x), __float_as_uint(gamma), 0x80000000u, 0x78)) > threshold;   // x ^ (gamma & sign)
