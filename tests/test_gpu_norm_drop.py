@@ -711,3 +711,19 @@ def test_relu_gate_without_deviation(ua, dtype, shape):
                                            rnd(3, C).cuda(), beta.cuda(), act="relu")
     assert torch.equal(db.cpu(), (beta > 0).float() * (B * H * W))            # counts below 2^24: exact
     assert (dw == 0).all() and (dx == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 8, 8, 64, 8), (3, 1, 2, 64, 64), (2, 128, 128, 40, 5), (1, 256, 255, 66, 3)])
+def test_relu_gate_of_groups_without_deviations(ua, dtype, shape):
+    """x is the mean throughout, so z = beta: also where beta / (rstd gamma) is nothing next to the mean, in 64 bits too."""
+    B, H, W, C, G = shape
+    mean = torch.tensor([5.25, -5.25, 2.0 ** 60, -2.0 ** 60, 1.5e-3, 2.0 ** -70])[torch.arange(B * G) % 6].to(dtype).float().view(B, G)
+    x = N._per_channel(mean, C // G).expand(B, H, W, C).contiguous()
+    beta = rnd(2, C) * torch.tensor([1e-18, 1.0, 1e-30])[torch.arange(C) % 3]
+    gamma = rnd(3, C)
+    dy = torch.ones(B, H, W, C)
+    rstd = torch.full((B, G), 1e-5).rsqrt()
+    dx, dw, db = ua.ops.group_norm_act_bwd(place(x, dtype), place(dy, dtype), mean.cuda(), rstd.cuda(), C, G, gamma.cuda(), beta.cuda(),
+                                           act="relu")
+    assert torch.equal(db.cpu(), (beta > 0).float() * (B * H * W)) and (dw == 0).all()

@@ -856,7 +856,8 @@ __global__ __launch_bounds__(kThreads) void gn_bwd_apply_kernel(const NormArgs a
 }
 // ReLU's gate is a border that fp32 rounding of z may cross.  But z > 0 is  sign(gamma) x > sign(gamma) tau  with
 // tau = mean - beta / (rstd gamma), and x is an fp32 value: against tau in 64 bits, rounded down to fp32, the comparison is
-// exact.  A channel's tau is worked out once per workgroup; the gate costs two instructions and needs no z.
+// exact.  Where x is the mean, as in a group without deviations, z = beta: its sign decides, also where nothing is left of the
+// quotient next to the mean.  A channel's tau is worked out once per workgroup; the gate costs two instructions and needs no z.
 // The quotient by two steps of Newton's method from the hardware's reciprocal (a library division works a special case per
 // operand out besides, one after the other).
 __device__ __forceinline__ float relu_threshold(float mean, float rstd, float gamma, float beta) {
@@ -868,7 +869,8 @@ __device__ __forceinline__ float relu_threshold(float mean, float rstd, float ga
   tau = gamma < 0.f ? -tau : tau;
   const float f = (float)tau;
   const float below = f > 0.f ? __uint_as_float(__float_as_uint(f) - 1) : __uint_as_float(f < 0.f ? __float_as_uint(f) + 1 : 0x80000001u);
-  const float t = (double)f > tau ? below : f;                   // f itself where tau is an fp32 value, infinite or NaN
+  const bool down = f == (gamma < 0.f ? -mean : mean) ? beta > 0.f : (double)f > tau;
+  const float t = down ? below : f;                              // f itself where tau is an fp32 value, infinite or NaN
   return d == 0.0 ? (beta > 0.f ? -INFINITY : INFINITY) : t;     // z = beta
 }
 __device__ __forceinline__ bool relu_gate(float x, float gamma, float threshold) {
@@ -889,7 +891,10 @@ __device__ __forceinline__ void relu_thresholds(const Slab& s, const SlabThread&
                                                 const float* gamma, const float* beta, float* shared, float* out) {
   if (s.rows < N) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) out[j] = relu_threshold(mean[j * NS / N], rstd[j * NS / N], gamma[j], beta[j]);
+    for (int j = 0; j < N; ++j) {
+      out[j] = relu_threshold(mean[j * NS / N], rstd[j * NS / N], gamma[j], beta[j]);
+      asm volatile("" : "+v"(out[j]));                           // one after the other: eight at a time need the tile's registers
+    }
     return;
   }
   float* mine = shared + t.slot * s.lanes * N;
