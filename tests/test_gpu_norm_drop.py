@@ -727,3 +727,26 @@ def test_relu_gate_of_groups_without_deviations(ua, dtype, shape):
     dx, dw, db = ua.ops.group_norm_act_bwd(place(x, dtype), place(dy, dtype), mean.cuda(), rstd.cuda(), C, G, gamma.cuda(), beta.cuda(),
                                            act="relu")
     assert torch.equal(db.cpu(), (beta > 0).float() * (B * H * W)) and (dw == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", LARGE)
+@pytest.mark.parametrize("kind", ACTS)
+def test_norm_backward_of_large_values(ua, monkeypatch, dtype, shape, kind):
+    """Deviations whose squares fp32 does not hold: dx keeps all three of its terms."""
+    B, H, W, C, G = shape
+    ops = ua.ops
+    scale, shift = grouped([1.0, 1e18, 1e25, 2e36], B, C, G), grouped([0.0, 0.0, 1e27, 0.0, 1.0, 1e20], B, C, G)
+    x = ((rnd(1, B, H, W, C) + rnd(2, C)) * scale + shift).to(dtype)
+    dy = rnd(5, B, H, W, C, scale=0.1).to(dtype)
+    gamma, beta = rnd(3, C, scale=0.3, shift=1.0), rnd(4, C, scale=0.3)
+    x6, g6, b6 = x.double(), gamma.double(), beta.double()
+    _, om, orr, _ = N.group_norm_act_fwd(x6, G, g6, b6, kind, 1e-5)
+    m, r = om.float(), orr.float()
+
+    def call():
+        return ops.group_norm_act_bwd(place(x, dtype), place(dy, dtype), m.cuda(), r.cuda(), C, G, gamma.cuda(), beta.cuda(), act=kind)
+    out = call()
+    bwd_check(out, x6, dy.double(), m.double(), r.double(), G, g6, b6, kind, None, dtype, f"{shape} {kind}")
+    monkeypatch.setattr(ops, "_POLLS", 0)
+    assert all(torch.equal(s, t) for s, t in zip(out, call()))

@@ -923,6 +923,19 @@ template <int NS, int N> __device__ __forceinline__ void slab_scale(const float*
 #pragma unroll
   for (int j = 0; j < N; ++j) scaled[j] *= rstd[j * NS / N];
 }
+// x in units of a power of two near the group's standard deviation, where that is above 1: mean and rstd in these units, and
+// the unit's inverse.  Squares of rstd and sums of x would leave fp32's range otherwise (at deviations of 10^20 dx lost its
+// third term); a power of two changes no other bit.
+template <int NS> __device__ __forceinline__ void slab_units(float* mean, float* rstd, float* unit) {
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const uint32_t power = __float_as_uint(rstd[j]) & 0x7f800000u;                     // 2^floor(log2 rstd), 0 of a subnormal rstd
+    const bool in = power > 0 && rstd[j] < 1.f;
+    unit[j] = in ? __uint_as_float(power) : 1.f;
+    mean[j] *= unit[j];
+    rstd[j] *= in ? __uint_as_float(0x7f000000u - power) : 1.f;
+  }
+}
 // Publishes a part's two sums of each group.
 template <int NS, int N>
 __device__ __forceinline__ void publish_bwd(const NormArgs& a, const SlabThread& t, int part, const float (&sum)[2][NS]) {
@@ -965,12 +978,13 @@ __device__ __forceinline__ void store_channel(const NormArgs& a, int row, int c,
   if (a.dgamma) a.dgamma[c] = a.ga * sum_dzh + (a.gb != 0.f ? a.gb * a.dgamma[c] : 0.f);
   if (a.dbeta) a.dbeta[c] = a.ga * sum_dz + (a.gb != 0.f ? a.gb * a.dbeta[c] : 0.f);
 }
-// Adds a vector's dz and dz * (x - mean) to the sums of its channels (d4: dy, dropped units cleared; scaled: gamma * rstd).
+// Adds a vector's dz and dz * (x - mean) to the sums of its channels (d4: dy, dropped units cleared; scaled: gamma * rstd; x as
+// slab_units has it).
 // What the second pass needs of dy comes back: with gated-off units cleared; in fp32 as dz itself, and so in bf16 with
 // SPLIT, the upper halves of dz in d4, the lower ones in `low` (else its slope is worked out again: a bf16 dz would be rounded).
 template <typename T, int NS, int ACT, bool SPLIT>
-__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, u32x4_t& low, const float* mean, const float* scaled, const float* beta,
-                                         const float* threshold, float* ch) {
+__device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, u32x4_t& low, const float* mean, const float* unit, const float* scaled,
+                                         const float* beta, const float* threshold, float* ch) {
   constexpr int N = ActVec<T>::N;
 #pragma unroll
   for (int e = 0; e < N / 4; ++e) {
@@ -984,7 +998,7 @@ __device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, u32x4_t& low, 
       if (e == N / 4 - 1) pin(d4, mean[0]);                      // what was packed is not kept unpacked besides
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] -= mean[(4 * e + j) * NS / N];
+    for (int j = 0; j < 4; ++j) x[j] = fmaf(x[j], unit[(4 * e + j) * NS / N], -mean[(4 * e + j) * NS / N]);
     if constexpr (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[4 * e + j], beta[4 * e + j]));
@@ -1022,10 +1036,11 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
   const NormGeom& g = a.g;
   const SlabPixels px = slab_pixels<I>(t, g, s, part);
   const int c0 = opaque(t.v * N), chunk_c0 = t.chunk * s.cv * N;
-  float mean[NS], rstd[NS], scaled[N], beta[N], threshold[N], ch[2 * N] = {}, sum[2][NS];
+  float mean[NS], rstd[NS], unit[NS], scaled[N], beta[N], threshold[N], ch[2 * N] = {}, sum[2][NS];
   slab_channels<NS, N>(a, t.b, c0, mean, rstd, scaled, beta);
   if constexpr (ACT == MI_ACT_RELU)
     relu_thresholds<NS, N>(s, t, relu_inputs(a, t, chunk_c0, t.tin), mean, rstd, scaled, beta, shared, threshold);
+  slab_units<NS>(mean, rstd, unit);
   slab_scale<NS, N>(rstd, scaled);
   const auto x = in_memory<T, I>(t, px, g, s, a.x, a.xcs, a.xco), dy = in_memory<T, I>(t, px, g, s, a.dy, a.ycs, a.yco);
 #pragma unroll 1
@@ -1038,7 +1053,7 @@ __device__ __forceinline__ void bwd_other_part(const NormArgs& a, const Slab& s,
       d = keep.kept(0, d);
     }
     u32x4_t unused;
-    bwd_step<T, NS, ACT, false>(x(i, 0.f), d, unused, mean, scaled, beta, threshold, ch);
+    bwd_step<T, NS, ACT, false>(x(i, 0.f), d, unused, mean, unit, scaled, beta, threshold, ch);
   }
   bwd_group_sums<NS, N>(ch, scaled, sum);
   slab_sum<NS, 2>(sum, g, s, t, shared);
@@ -1126,11 +1141,11 @@ __device__ __forceinline__ void bwd_means(const NormArgs& a, const Slab& s, cons
   }
 }
 // dx of a part from the registers:  dx = scaled * dz - M1 - (x - mean) * rstd^2 * M2,  M1 and M2 the means over the group of
-// scaled * dz and scaled * dz * (x - mean); times dropout's factor.
+// scaled * dz and scaled * dz * (x - mean); times dropout's factor, and by the unit of x.
 template <typename T, int NS, int I, int ACT, bool SPLIT>
 __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const SlabThread& t, const SlabPixels& px, u32x4_t (&vx)[I],
-                                         u32x4_t (&vd)[I], const u32x4_t* low, const float* mean, const float* rstd, const float* scaled, const float* beta,
-                                         const float (&sum)[2][NS], float factor) {
+                                         u32x4_t (&vd)[I], const u32x4_t* low, const float* mean, const float* rstd, const float* unit, const float* scaled,
+                                         const float* beta, const float (&sum)[2][NS], float factor) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
   const int c0 = t.v * N;
   T* out = (T*)a.out + ((int64_t)t.b * a.g.P + px.first + t.row) * a.ocs + a.oco + c0;
@@ -1140,11 +1155,11 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
   float b0[NS], b1[NS], slope[N];
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    b0[j] = -sum[0][j] * factor;
-    b1[j] = -sum[1][j] * rstd[j] * rstd[j] * factor;
+    b0[j] = -sum[0][j] * (factor * unit[j]);
+    b1[j] = -sum[1][j] * rstd[j] * rstd[j] * (factor * unit[j]);
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) slope[j] = scaled[j] * factor;
+  for (int j = 0; j < N; ++j) slope[j] = scaled[j] * (factor * unit[j / Q]);
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     pin(vx[i], sum[0][0]);
@@ -1160,7 +1175,7 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = 4 * e + j, k = c / Q;
-        x[j] -= mean[k];
+        x[j] = fmaf(x[j], unit[k], -mean[k]);
         if constexpr (N == 8 && !SPLIT && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[c], beta[c]));
         d[j] = fmaf(x[j], b1[k], fmaf(d[j], slope[c], b0[k]));
       }
@@ -1198,13 +1213,14 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
   const float scale = a.drop.on ? a.drop.scale : 1.f;
   const SlabPixels px = slab_pixels<I>(t, g, s, t.part);
   u32x4_t vx[I], vd[I];
-  float mean[NS], rstd[NS], scaled[N], beta[N], threshold[N], sum[2][NS], ch[2 * N] = {};
+  float mean[NS], rstd[NS], unit[NS], scaled[N], beta[N], threshold[N], sum[2][NS], ch[2 * N] = {};
   ReluInputs first;
   if constexpr (ACT == MI_ACT_RELU) first = relu_inputs(a, t, t.chunk * s.cv * N, t.tin);
   slab_channels<NS, N>(a, t.b, c0, mean, rstd, scaled, beta);
   load_slab<T, I>(t, px, g, s, a.x, a.xcs, a.xco, vx);
   load_slab<T, I>(t, px, g, s, a.dy, a.ycs, a.yco, vd);
   if constexpr (ACT == MI_ACT_RELU) relu_thresholds<NS, N>(s, t, first, mean, rstd, scaled, beta, shared, threshold);
+  slab_units<NS>(mean, rstd, unit);
   slab_scale<NS, N>(rstd, scaled);
   bwd_drop<T, I>(a, s, t, px, vd);
   zero_missing(px, vx);
@@ -1214,7 +1230,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
     pin(vx[i], scaled[0]);
     pin(vd[i], scaled[0]);
     u32x4_t lo;
-    bwd_step<T, NS, ACT, SPLIT>(vx[i], vd[i], lo, mean, scaled, beta, threshold, ch);
+    bwd_step<T, NS, ACT, SPLIT>(vx[i], vd[i], lo, mean, unit, scaled, beta, threshold, ch);
     if constexpr (SPLIT) low[i * kSlabThreads + threadIdx.x] = lo;
   }
   bwd_group_sums<NS, N>(ch, scaled, sum);
@@ -1226,9 +1242,10 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
   bwd_means<T, NS, I, PARTS, ACT>(a, s, t, sum, shared);
   if constexpr (PARTS) {                                         // the exchange needs their registers
     slab_channels<NS, N>(a, t.b, opaque(c0), mean, rstd, scaled, beta);
+    slab_units<NS>(mean, rstd, unit);
     slab_scale<NS, N>(rstd, scaled);
   }
-  bwd_emit<T, NS, I, ACT, SPLIT>(a, s, t, px, vx, vd, low + threadIdx.x, mean, rstd, scaled, beta, sum, scale);
+  bwd_emit<T, NS, I, ACT, SPLIT>(a, s, t, px, vx, vd, low + threadIdx.x, mean, rstd, unit, scaled, beta, sum, scale);
 }
 // ---------------------------------------------------------------- launches
 // in norm.hip
