@@ -166,3 +166,10 @@ def test_modules_carry_group_norms_parameters(ua):
     a = [ua.layers.fresh_drop(0.5).seed for _ in range(3)]
     torch.manual_seed(5)
     assert a == [ua.layers.fresh_drop(0.5).seed for _ in range(3)] and len(set(a)) == 3
+
+
+def test_dropout_module_without_drops_needs_the_kernels_for_other_widths(ua):
+    d = ua.Dropout(40, 0.5).eval()
+    for args in ((torch.zeros(2, 4, 4, 48), torch.zeros(2, 4, 4, 64)), (torch.zeros(2, 4, 4, 64),)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            d(*args)

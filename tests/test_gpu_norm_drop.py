@@ -750,3 +750,28 @@ def test_norm_backward_of_large_values(ua, monkeypatch, dtype, shape, kind):
     bwd_check(out, x6, dy.double(), m.double(), r.double(), G, g6, b6, kind, None, dtype, f"{shape} {kind}")
     monkeypatch.setattr(ops, "_POLLS", 0)
     assert all(torch.equal(s, t) for s, t in zip(out, call()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("p, training", [(0.5, False), (0.0, True), (0.0, False)])
+def test_dropout_module_that_drops_nothing(ua, dtype, p, training):
+    """Evaluation mode takes the widths that training mode takes and returns what it returns: padded channels, padding zero."""
+    B, H, W, C = 2, 5, 6, 40
+    d = ua.Dropout(C, p).train(training)
+    x, r, dy = rnd(1, B, H, W, C).to(dtype), rnd(2, B, H, W, C).to(dtype), rnd(3, B, H, W, C).to(dtype)
+    want = (x.double() + r.double()).to(dtype)
+    for xa, ra in ((0, 16), (16, 0), (0, 0), (32, 16)):
+        xb, rb = place(x, dtype, after=xa, fill=3.0).requires_grad_(), place(r, dtype, after=ra, fill=5.0).requires_grad_()
+        y = d(xb, rb)
+        assert y.shape == (B, H, W, 48) and y.dtype == dtype and torch.equal(y[..., :C].cpu(), want)
+        check_padding(y, C)
+        gx, gr = torch.autograd.grad(y, (xb, rb), place(dy, dtype, fill=7.0))
+        for g, leaf in ((gx, xb), (gr, rb)):
+            assert g.shape == leaf.shape and torch.equal(g[..., :C].cpu(), dy) and (g[..., C:] == 0).all()
+    wide, narrow = place(x, dtype, after=16, fill=3.0), place(x, dtype, fill=3.0)
+    y = d(wide)
+    assert y.shape == (B, H, W, 48) and torch.equal(y[..., :C].cpu(), x)
+    check_padding(y, C)
+    assert d(narrow) is narrow
+    with pytest.raises(ValueError, match="does not go with"):
+        d(narrow, narrow.double())

@@ -65,8 +65,8 @@ def group_norm_act(x, channels: int, groups: int, weight=None, bias=None, act: s
     return _GroupNormActFunction.apply(x, weight, bias, channels, groups, act, eps, drop)
 
 
-def dropout(x, channels: int, drop: ops.Drop, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``residual + dropout(x)``, differentiable in both."""
+def dropout(x, channels: int, drop: Optional[ops.Drop], residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``residual + dropout(x)``, differentiable in both; without a ``drop`` nothing is dropped."""
     return _DropoutFunction.apply(x, residual, channels, drop)
 
 
@@ -77,7 +77,8 @@ def fresh_drop(p: float, per_channel: bool = False, offset_dev: Optional[torch.T
 
 
 class Dropout(nn.Module):
-    """``residual + dropout(x)`` in training mode, ``residual + x`` in evaluation mode.
+    """``residual + dropout(x)`` in training mode, ``residual + x`` in evaluation mode and where ``p`` is 0: by the same
+    operator, so inputs may be wider than the channels in both, and differently wide.
 
     ``offset_dev``: a one-element int64 GPU tensor for steps captured into a graph, whose seed is fixed by the capture;
     the caller counts it up once per step, after the backward pass."""
@@ -89,9 +90,13 @@ class Dropout(nn.Module):
         self.channels, self.p, self.per_channel, self.offset_dev = int(channels), float(p), bool(per_channel), offset_dev
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if not self.training or self.p == 0.0:
-            return x if residual is None else x + residual
-        return dropout(x, self.channels, fresh_drop(self.p, self.per_channel, self.offset_dev), residual)
+        if self.training and self.p > 0.0:
+            return dropout(x, self.channels, fresh_drop(self.p, self.per_channel, self.offset_dev), residual)
+        if residual is None and x.shape[-1] == ops.pad_ch(self.channels):
+            return x
+        if residual is not None and not x.is_cuda and x.shape == residual.shape:       # nothing is dropped, and there are no kernels
+            return x + residual
+        return dropout(x, self.channels, None, residual)
 
     def extra_repr(self) -> str:
         return f"{self.channels}, p={self.p}, per_channel={self.per_channel}"
