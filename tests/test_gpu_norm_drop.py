@@ -775,3 +775,17 @@ def test_dropout_module_that_drops_nothing(ua, dtype, p, training):
     assert d(narrow) is narrow
     with pytest.raises(ValueError, match="does not go with"):
         d(narrow, narrow.double())
+
+
+def test_a_counter_changed_between_forward_and_backward_is_reported(ua):
+    """Two forward passes with the count between them and one backward pass: the first one's mask is gone."""
+    C, step = 64, torch.zeros(1, dtype=torch.int64, device="cuda")
+    norm, drop = ua.GroupNormAct(8, C, p=0.5, offset_dev=step).cuda(), ua.Dropout(C, 0.5, offset_dev=step)
+    for layer in (norm, drop):
+        x = rnd(1, 2, 4, 4, C).cuda().requires_grad_()
+        first = layer(x)
+        step.add_(1)
+        second = layer(x)
+        torch.autograd.grad(second.sum(), x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(first.sum(), x)

@@ -23,18 +23,24 @@ def _widened(d: torch.Tensor, width: int) -> torch.Tensor:
     return d if d.shape[3] == width else torch.nn.functional.pad(d, (0, width - d.shape[3]))
 
 
+def _counter(drop: Optional[ops.Drop]) -> Optional[torch.Tensor]:
+    """What a drop reads on the device when a kernel runs.  Saved for backward: autograd then reports a counter that was
+    changed between the two passes, whose masks would differ."""
+    return drop.offset_dev if drop is not None else None
+
+
 class _GroupNormActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, channels, groups, act, eps, drop):
         y, mean, rstd = ops.group_norm_act_fwd(x, channels, groups, weight, bias, act=act, eps=eps, drop=drop)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.save_for_backward(x, weight, bias, mean, rstd, _counter(drop))
         ctx.spec = channels, groups, act, drop
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        x, weight, bias, mean, rstd, _ = ctx.saved_tensors
         channels, groups, act, drop = ctx.spec
         dx, dweight, dbias = ops.group_norm_act_bwd(x, _grad(dy, x), mean, rstd, channels, groups, weight, bias, act=act, drop=drop)
         return _widened(dx, x.shape[3]), dweight, dbias, None, None, None, None, None
@@ -43,6 +49,7 @@ class _GroupNormActFunction(torch.autograd.Function):
 class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, channels, drop):
+        ctx.save_for_backward(_counter(drop))
         ctx.spec, ctx.width = (channels, drop), x.shape[3]
         ctx.residual_width = residual.shape[3] if residual is not None else 0
         return ops.dropout_fwd(x, channels, drop, residual=residual)
@@ -50,6 +57,7 @@ class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _ = ctx.saved_tensors                      # raises where the counter was changed
         channels, drop = ctx.spec
         dy = dy.contiguous()
         dx = _widened(ops.dropout_bwd(dy, channels, drop), ctx.width) if ctx.needs_input_grad[0] else None
