@@ -173,3 +173,13 @@ def test_dropout_module_without_drops_needs_the_kernels_for_other_widths(ua):
     for args in ((torch.zeros(2, 4, 4, 48), torch.zeros(2, 4, 4, 64)), (torch.zeros(2, 4, 4, 64),)):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             d(*args)
+
+
+def test_a_drop_is_fixed(ua):
+    """Setting an attribute had no effect on what the kernels were given."""
+    drop = ua.ops.Drop(0.5, 1, 2, per_channel=True)
+    for name, value in (("p", 0.1), ("seed", 3), ("offset", 4), ("offset_dev", None), ("per_channel", False)):
+        with pytest.raises(AttributeError):
+            setattr(drop, name, value)
+    assert (drop.p, drop.seed, drop.offset, drop.offset_dev, drop.per_channel) == (0.5, 1, 2, None, True)
+    assert (drop._desc.p, drop._desc.seed, drop._desc.offset, drop._desc.per_channel) == (0.5, 1, 2, 1)

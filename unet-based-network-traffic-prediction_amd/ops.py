@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -221,9 +222,11 @@ class Drop:
     ``p`` counts in steps of 2^-16 (survivors are scaled by the rounded value).  ``seed`` and ``offset`` are integers
     in [0, 2^64); layers of one step take different offsets (or seeds).  ``offset_dev`` (a one-element int64 tensor on
     the GPU) is added to ``offset`` when a kernel runs: a captured graph replays with new masks if it is counted up
-    between replays.  ``per_channel`` drops whole feature maps."""
+    between replays.  ``per_channel`` drops whole feature maps.  A ``Drop`` is fixed once it is made: a backward pass that is
+    still to come needs it as it was."""
 
-    __slots__ = ("p", "seed", "offset", "offset_dev", "per_channel", "_desc")
+    __slots__ = ("_p", "_seed", "_offset", "_offset_dev", "_per_channel", "_desc")
+    p, seed, offset, offset_dev, per_channel = (property(operator.attrgetter(n)) for n in __slots__[:-1])
 
     def __init__(self, p: float, seed: int, offset: int = 0, offset_dev: Optional[torch.Tensor] = None,
                  per_channel: bool = False):
@@ -233,15 +236,15 @@ class Drop:
             raise ValueError("dropout: seed and offset must be in [0, 2^64)")
         if offset_dev is not None and (offset_dev.dtype != torch.int64 or offset_dev.numel() != 1 or not offset_dev.is_cuda):
             raise ValueError("dropout: offset_dev must be a one-element int64 tensor on the GPU")
-        self.p, self.seed, self.offset, self.offset_dev, self.per_channel = p, seed, offset, offset_dev, per_channel
+        self._p, self._seed, self._offset, self._offset_dev, self._per_channel = p, seed, offset, offset_dev, per_channel
         self._desc = _DropoutDesc(p, seed, offset, offset_dev.data_ptr() if offset_dev is not None else None, int(per_channel))
 
 
 def _drop_ref(drop: Optional[Drop], dev: torch.device):
     if drop is None:
         return None
-    if drop.offset_dev is not None and drop.offset_dev.device != dev:
-        raise RuntimeError(f"dropout: offset_dev is on {drop.offset_dev.device}, the activation on {dev}")
+    if drop._offset_dev is not None and drop._offset_dev.device != dev:
+        raise RuntimeError(f"dropout: offset_dev is on {drop._offset_dev.device}, the activation on {dev}")
     return ctypes.byref(drop._desc)
 
 
