@@ -789,3 +789,20 @@ def test_a_counter_changed_between_forward_and_backward_is_reported(ua):
         torch.autograd.grad(second.sum(), x)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(first.sum(), x)
+
+
+@pytest.mark.parametrize("frozen", [("weight",), ("bias",), ("weight", "bias")])
+def test_frozen_parameters_cost_no_sums(ua, monkeypatch, frozen):
+    """Gradients that nobody asked for are not worked out; the others are the same bits."""
+    ops, made = ua.ops, []
+    bwd = ops.group_norm_act_bwd
+    monkeypatch.setattr(ops, "group_norm_act_bwd", lambda *a, **k: made.append(bwd(*a, **k)) or made[-1])
+    norm = ua.GroupNormAct(8, 64, act="silu").cuda()
+    x, dy = rnd(1, 40, 16, 16, 64).cuda().requires_grad_(), rnd(2, 40, 16, 16, 64).cuda()
+    every = torch.autograd.grad(norm(x), (x, norm.weight, norm.bias), dy)
+    for name in frozen:
+        getattr(norm, name).requires_grad_(False)
+    norm(x).backward(dy)
+    assert torch.equal(x.grad, every[0])
+    for name, got, want in zip(("weight", "bias"), made[-1][1:], every[1:]):
+        assert got is None and getattr(norm, name).grad is None if name in frozen else torch.equal(got, want)

@@ -42,7 +42,8 @@ class _GroupNormActFunction(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, mean, rstd, _ = ctx.saved_tensors
         channels, groups, act, drop = ctx.spec
-        dx, dweight, dbias = ops.group_norm_act_bwd(x, _grad(dy, x), mean, rstd, channels, groups, weight, bias, act=act, drop=drop)
+        dx, dweight, dbias = ops.group_norm_act_bwd(x, _grad(dy, x), mean, rstd, channels, groups, weight, bias, act=act, drop=drop,
+                                                    want_dweight=ctx.needs_input_grad[1], want_dbias=ctx.needs_input_grad[2])
         return _widened(dx, x.shape[3]), dweight, dbias, None, None, None, None, None
 
 

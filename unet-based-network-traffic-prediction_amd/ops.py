@@ -363,9 +363,9 @@ def group_norm_act_fwd(x, C, groups, weight=None, bias=None, act="none", eps=1e-
 
 
 def group_norm_act_bwd(x, dy, mean, rstd, C, groups, weight=None, bias=None, act="none", drop: Optional[Drop] = None, x_coff=0,
-                       dy_coff=0, dweight=None, dbias=None, alpha=1.0, beta=0.0):
+                       dy_coff=0, dweight=None, dbias=None, alpha=1.0, beta=0.0, want_dweight=True, want_dbias=True):
     """(dx, dweight, dbias) from what the forward pass was given and returned.  ``dweight`` / ``dbias`` are None where
-    the parameter is; tensors passed in receive ``alpha * gradient + beta * themselves``."""
+    the parameter is, or is not wanted; tensors passed in receive ``alpha * gradient + beta * themselves``."""
     _nhwc(x, "group_norm_act")
     _nhwc(dy, "group_norm_act dy", x)
     B, H, W, cs = x.shape
@@ -377,9 +377,9 @@ def group_norm_act_bwd(x, dy, mean, rstd, C, groups, weight=None, bias=None, act
     mp, rp = (_channel_vector(t, B * groups, dev, "group_norm_act statistics") for t in (mean, rstd))
     with _on(dev):
         dx = _new_activation(x, C)
-        if weight is not None and dweight is None:
+        if weight is not None and dweight is None and want_dweight:
             dweight = torch.empty_like(weight) if beta == 0.0 else torch.zeros_like(weight)
-        if bias is not None and dbias is None:
+        if bias is not None and dbias is None and want_dbias:
             dbias = torch.empty_like(bias) if beta == 0.0 else torch.zeros_like(bias)
         gp, hp = _channel_vector(dweight, C, dev, "group_norm_act dweight"), _channel_vector(dbias, C, dev, "group_norm_act dbias")
         nbytes = _norm_ws_bytes(B, H, W, C, groups, 1, dt)
