@@ -183,3 +183,11 @@ def test_a_drop_is_fixed(ua):
             setattr(drop, name, value)
     assert (drop.p, drop.seed, drop.offset, drop.offset_dev, drop.per_channel) == (0.5, 1, 2, None, True)
     assert (drop._desc.p, drop._desc.seed, drop._desc.offset, drop._desc.per_channel) == (0.5, 1, 2, 1)
+
+
+def test_many_rows_in_one_group_are_taken(ua):
+    """5 million rows of 528 channels: refused for the workspace alone, not for joins with more threads than they run with."""
+    L, far = ua.lib(), 1 << 45
+    assert _norm_fwd(L, B=5_000_000, H=1, W=1, Cc=528, G=1, xcs=528, ycs=528, y=far, dt=1, ws_bytes=8) == -2
+    assert L.mi_group_norm_act_bwd(A, 528, 0, far, 528, 0, None, None, A, A, far << 1, 528, 0, None, None, 1.0, 0.0, 5_000_000, 1, 1, 528, 1,
+                                   1, None, -1, A, 8, 1, None) == -2

@@ -806,3 +806,30 @@ def test_frozen_parameters_cost_no_sums(ua, monkeypatch, frozen):
     assert torch.equal(x.grad, every[0])
     for name, got, want in zip(("weight", "bias"), made[-1][1:], every[1:]):
         assert got is None and getattr(norm, name).grad is None if name in frozen else torch.equal(got, want)
+
+
+def test_millions_of_rows_in_one_group(ua):
+    """4.3 million images of one pixel with groups of more than 64 vectors: joins with a wave each, as a launch holds no more.
+    The last rows against the definition, the parameters' gradients against sums in 64 bits."""
+    ops, rows, C, tail = ua.ops, (1 << 22) + 100_001, 528, 1000
+    x = torch.empty((rows, 1, 1, C), device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator("cuda").manual_seed(1))
+    y, mean, rstd = ops.group_norm_act_fwd(x, C, 1, act="silu")
+    x6 = x[-tail:].double().cpu()
+    one, zero = torch.ones(C).double(), torch.zeros(C).double()
+    oy, om, orr, z = N.group_norm_act_fwd(x6, 1, one, zero, "silu", float(torch.tensor(1e-5)))
+    within(y[-tail:], oy, fwd_bound(x6, oy, z, om, orr, one, zero, 1, torch.bfloat16), "tail")
+    dx, dw, db = ops.group_norm_act_bwd(x, y, mean, rstd, C, 1, one.float().cuda(), zero.float().cuda(), act="none")
+    m, r = mean[-tail:].double().cpu(), rstd[-tail:].double().cpu()
+    bwd_check((dx[-tail:], None, None), x6, y[-tail:].double().cpu(), m, r, 1, one, zero, "none", None, torch.bfloat16, "tail")
+    want_w, want_b, size_w, size_b = (torch.zeros(C, device="cuda", dtype=torch.float64) for _ in range(4))
+    for k in range(0, rows, 1 << 18):
+        d = y[k:k + (1 << 18), 0, 0].double()
+        h = (x[k:k + (1 << 18), 0, 0].double() - mean[k:k + (1 << 18)].double()) * rstd[k:k + (1 << 18)].double()
+        want_w += (d * h).sum(0)
+        want_b += d.sum(0)
+        size_w += (d * h).abs().sum(0)
+        size_b += d.abs().sum(0)
+    within(dw, want_w.cpu(), ((K + 8) * U * size_w).cpu(), "dweight")
+    within(db, want_b.cpu(), (K * U * size_b).cpu(), "dbias")
+    del x, y, dx
+    torch.cuda.empty_cache()

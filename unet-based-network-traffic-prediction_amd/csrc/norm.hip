@@ -25,7 +25,6 @@ template <typename F> __device__ __forceinline__ F block_total(F v, F* shared) {
 // Joins the tiles and pieces of a group.  Piece k of an image's tile covers channels k*q .. k*q + q - 1.  One wave, or 1024
 // threads where there are many: a wave takes a memory latency for every 64 (22 images of 75x41x617 fp32 in one group, 60,000
 // pieces each, 576 us forward with one wave, 145 so; 9 of 64x64x1024 backward, channels along the threads, 626 and 152).
-constexpr int kJoinThreads = 1024;
 __global__ __launch_bounds__(kJoinThreads) void gn_join_kernel(const NormArgs a) {
   __shared__ double shared[kJoinThreads / 64];
   const NormGeom& g = a.g;
@@ -123,11 +122,10 @@ void launch_gn_empty(uint64_t* words, int64_t n, hipStream_t s) {
   hipLaunchKernelGGL(gn_empty_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s, words, n);
 }
 void launch_gn_join(const NormArgs& a, hipStream_t s) {
-  const bool many = (int64_t)a.g.tiles * (a.g.cg / a.g.q) > 512;
-  hipLaunchKernelGGL(gn_join_kernel, dim3(a.g.B * a.g.G), dim3(many ? kJoinThreads : 64), 0, s, a);
+  hipLaunchKernelGGL(gn_join_kernel, dim3(a.g.B * a.g.G), dim3(join_threads(a.g, false)), 0, s, a);
 }
 void launch_gn_bwd_join(const NormArgs& a, int padded, hipStream_t s) {
-  hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.g.B * a.g.G), dim3(a.g.cg > 64 ? kJoinThreads : 64), 0, s, a, padded);
+  hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.g.B * a.g.G), dim3(join_threads(a.g, true)), 0, s, a, padded);
 }
 void launch_gn_param_grads(const NormArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(gn_param_grads_kernel, dim3((a.g.C + 7) / 8), dim3(1024), 0, s, a);
@@ -157,9 +155,9 @@ static int check_range(const NormGeom& g, const char* what) {
   return MI_OK;
 }
 // A launch holds less than 2^32 threads.
-static int check_threads(const NormGeom& g, const Slab* s, const char* what) {
+static int check_threads(const NormGeom& g, const Slab* s, bool backward, const char* what) {
   const int64_t threads = s ? (int64_t)s->img_blocks * s->parts * s->chunks * s->threads
-                            : std::max((int64_t)g.B * g.tiles * g.chunks * kThreads, (int64_t)g.B * g.G * kJoinThreads);
+                            : std::max((int64_t)g.B * g.tiles * g.chunks * kThreads, (int64_t)g.B * g.G * join_threads(g, backward));
   MI_REQUIRE(threads < (1ll << 32), std::string(what) + ": tensor too large");
   return MI_OK;
 }
@@ -174,7 +172,7 @@ int launch_group_norm_fwd(const void* x, int xcs, int xco, const float* gamma, c
   if (B == 0) return MI_OK;
   Slab slab;
   const Slab* sl = choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, false, &slab) ? &slab : nullptr;
-  if ((rc = check_threads(a.g, sl, "group_norm_act_fwd"))) return rc;
+  if ((rc = check_threads(a.g, sl, false, "group_norm_act_fwd"))) return rc;
   if (polls >= 0) slab.polls = polls;
   if (ws_bytes < group_norm_ws_bytes(B, H, W, C, G, 0, dtype)) return fail(MI_ESIZE, "group_norm_act_fwd: workspace too small");
   a.x = x; a.xcs = xcs; a.xco = xco;
@@ -196,7 +194,7 @@ int launch_group_norm_bwd(const void* x, int xcs, int xco, const void* dy, int y
   if ((rc = check_range(a.g, "group_norm_act_bwd"))) return rc;
   Slab slab;
   const Slab* sl = B > 0 && choose_slab(a.g, dtype == MI_BF16 ? 8 : 4, true, &slab) ? &slab : nullptr;
-  if ((rc = check_threads(a.g, sl, "group_norm_act_bwd"))) return rc;
+  if ((rc = check_threads(a.g, sl, true, "group_norm_act_bwd"))) return rc;
   if (polls >= 0) slab.polls = polls;
   if (ws_bytes < group_norm_ws_bytes(B, H, W, C, G, 1, dtype)) return fail(MI_ESIZE, "group_norm_act_bwd: workspace too small");
   a.x = x; a.xcs = xcs; a.xco = xco;

@@ -82,6 +82,14 @@ inline int slab_bwd_floats(const NormGeom& g, const Slab& s, int ns, int N, bool
   return thresholds > floats ? thresholds : floats;
 }
 
+// Threads that join the tiles of an (image, group): one wave, or 1024 threads where there are many (norm.hip) and a launch holds
+// them -- less than 2^32.
+constexpr int kJoinThreads = 1024;
+inline int join_threads(const NormGeom& g, bool backward) {
+  const bool many = backward ? g.cg > 64 : (int64_t)g.tiles * (g.cg / g.q) > 512;
+  return many && (int64_t)g.B * g.G * kJoinThreads < (1ll << 32) ? kJoinThreads : 64;
+}
+
 inline unsigned slab_grid(const Slab& s) { return (unsigned)(s.img_blocks * s.parts * s.chunks); }
 // 64-bit words that the parts exchange
 inline int64_t slab_words(const NormGeom& g, const Slab& s) { return 2 * (int64_t)g.B * s.parts * g.G; }
