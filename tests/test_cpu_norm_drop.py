@@ -191,3 +191,13 @@ def test_many_rows_in_one_group_are_taken(ua):
     assert _norm_fwd(L, B=5_000_000, H=1, W=1, Cc=528, G=1, xcs=528, ycs=528, y=far, dt=1, ws_bytes=8) == -2
     assert L.mi_group_norm_act_bwd(A, 528, 0, far, 528, 0, None, None, A, A, far << 1, 528, 0, None, None, 1.0, 0.0, 5_000_000, 1, 1, 528, 1,
                                    1, None, -1, A, 8, 1, None) == -2
+
+
+def test_refused_shapes_need_no_workspace(ua):
+    """The size of a workspace is asked for before the call that would refuse the shape."""
+    L, big = ua.lib(), (1 << 31) - 1
+    for backward in (0, 1):
+        for dt in (0, 1):
+            for shape in ((1, 1, 1, big, 1), (1, 1, 1, (1 << 24) + 16, 1), (1 << 20, 1 << 10, 1 << 10, 64, 8), (big, 2, 1, 32, 4)):
+                assert L.mi_group_norm_ws_bytes(*shape, backward, dt) == 0
+        assert L.mi_group_norm_ws_bytes(2, 256, 255, 66, 3, backward, 2) == 0 and L.mi_group_norm_ws_bytes(2, 256, 255, 66, 3, backward, 1) > 0

@@ -587,7 +587,9 @@ int mi_dropout_fwd(const void* x, int xcs, int xco, const void* r, int rcs, int 
   return launch_dropout(x, xcs, xco, r, rcs, rco, y, ycs, yco, B, H, W, C, drop, dtype, (hipStream_t)s);
 }
 size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backward, int dtype) {
-  if (B < 0 || H <= 0 || W <= 0 || C <= 0 || groups <= 0 || C % groups || (int64_t)H * W >= (1ll << 31)) return 0;
+  // shapes that the operators refuse need none
+  if (B < 0 || H <= 0 || W <= 0 || C <= 0 || C > (1 << 24) || groups <= 0 || C % groups || (dtype != MI_F32 && dtype != MI_BF16)) return 0;
+  if ((int64_t)H * W >= (1ll << 31) || (int64_t)B * H * W >= (1ll << 31)) return 0;
   return group_norm_ws_bytes(B, H, W, C, groups, backward, dtype);
 }
 #define MI_NORM_ARGS(what)                                                                                               \
