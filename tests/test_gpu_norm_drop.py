@@ -833,3 +833,46 @@ def test_millions_of_rows_in_one_group(ua):
     within(db, want_b.cpu(), (K * U * size_b).cpu(), "dbias")
     del x, y, dx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape, bias", [((1, 512, 512, 96, 1), 0.0), ((2, 1024, 1024, 64, 1), 3.0), ((1, 1024, 1024, 33, 3), 1.0),
+                                         ((1 << 21, 1, 1, 32, 8), 0.0), ((300, 96, 96, 32, 4), 2.0)])
+def test_gradients_of_one_sign(ua, dtype, shape, bias):
+    """A constant dy, as the gradient of a sum is: thousands of tiles, rows or parts add to sums without any cancellation.  The
+    bounds are those of bwd_check with its K additions of 32 bits between an element and a sum; joins add in 64."""
+    B, H, W, C, G = shape
+    ops, gen = ua.ops, torch.Generator("cuda").manual_seed(1)
+    cg = C // G
+    x = torch.zeros((B, H, W, N.pad_ch(C)), device="cuda", dtype=dtype)
+    x[..., :C] = torch.randn(B, H, W, C, device="cuda", generator=gen)
+    dy = torch.full_like(x, 0.3)
+    gamma, beta = rnd(3, C, scale=0.3, shift=1.0).cuda(), (rnd(4, C, scale=0.3) + bias).cuda()
+    y, mean, rstd = ops.group_norm_act_fwd(x, C, G, gamma, beta, act="silu")
+    del y
+    dx, dw, db = ops.group_norm_act_bwd(x, dy, mean, rstd, C, G, gamma, beta, act="silu")
+    sums = [torch.zeros(C, device="cuda", dtype=torch.float64) for _ in range(4)]       # dweight, dbias and their bounds
+    step = max(1, (1 << 25) // (H * W * C))
+    for k in range(0, B, step):
+        b = slice(k, k + step)
+        x6, dy6 = x[b, ..., :C].double(), dy[b, ..., :C].double()
+        want, gw, gb, p = N.group_norm_act_bwd(x6, dy6, mean[b].double(), rstd[b].double(), G, gamma.double(), beta.double(), "silu")
+        ddz, dt = bwd_bounds(p, gamma.double(), beta.double(), dtype)
+        gm = lambda t: N._per_channel(N._group_mean(t, G), cg)
+        bound = p["r"] * (dt + gm(dt) + p["h"].abs() * gm(dt * p["h"].abs()) + K * U * (p["a1"] + p["h"].abs() * p["a2"])
+                          + 8 * U * (p["t"].abs() + p["m1"].abs() + (p["h"] * p["m2"]).abs())) + half_step(dtype) * want.abs() + 1e-37
+        assert ((dx[b, ..., :C].double() - want).abs() <= bound).all()
+        hb = p["h"].abs()
+        for s, t in zip(sums, (gw, gb, (ddz * hb + (K + 8) * U * (p["dz"] * p["h"]).abs()).sum((0, 1, 2)),
+                               (ddz + K * U * p["dz"].abs()).sum((0, 1, 2)))):
+            s += t
+    within(dw, sums[0].cpu(), sums[2].cpu() + 1e-37, "dweight")
+    within(db, sums[1].cpu(), sums[3].cpu() + 1e-37, "dbias")
+    del x, dy, dx
+    ones = torch.zeros((B, H, W, N.pad_ch(C)), device="cuda", dtype=dtype)
+    dy = torch.full_like(ones, 0.3)
+    _, _, db = ops.group_norm_act_bwd(ones, dy, mean, rstd, C, G, gamma, beta)
+    want = dy[0, 0, 0, 0].double().cpu() * (B * H * W)
+    within(db, want.expand(C), K * U * want.expand(C), "dbias of a constant")
+    del ones, dy
+    torch.cuda.empty_cache()

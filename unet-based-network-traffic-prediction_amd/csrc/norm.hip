@@ -53,50 +53,56 @@ __global__ __launch_bounds__(kJoinThreads) void gn_join_kernel(const NormArgs a)
     a.rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)a.eps));
   }
 }
-// One workgroup per (image, group): the image's sums of each channel, and the group's two means.
+// One workgroup per (image, group): the image's sums of each channel, and the group's two means.  In 64 bits: an image has
+// thousands of tiles, and their sums may all have one sign (8,192 tiles of a constant dy lost 10^-4 of dbias in 32 bits).
 __global__ __launch_bounds__(kJoinThreads) void gn_bwd_join_kernel(const NormArgs a, int padded) {
-  __shared__ float shared[kJoinThreads / 64];
+  __shared__ double shared[kJoinThreads / 64];
   const NormGeom& g = a.g;
   const int b = blockIdx.x / g.G, gi = blockIdx.x - b * g.G;
-  float m1 = 0.f, m2 = 0.f;
+  double m1 = 0.0, m2 = 0.0;
   for (int k = threadIdx.x; k < g.cg; k += blockDim.x) {
     const int c = gi * g.cg + k;
     const float2* part = a.part + (int64_t)b * g.tiles * padded + c;
-    float2 s = make_float2(0.f, 0.f);
+    double s0 = 0.0, s1 = 0.0;
 #pragma unroll 8
     for (int t = 0; t < g.tiles; ++t) {                          // eight loads under way, one order of the sums
       const float2 p = part[(int64_t)t * padded];
-      s.x += p.x;
-      s.y += p.y;
+      s0 += (double)p.x;
+      s1 += (double)p.y;
     }
-    a.chan[(int64_t)b * g.C + c] = s;
-    const float gamma = a.gamma != nullptr ? a.gamma[c] : 1.f;
-    m1 = fmaf(gamma, s.x, m1);
-    m2 = fmaf(gamma, s.y, m2);
+    a.chan[(int64_t)b * g.C + c] = make_float2((float)s0, (float)s1);
+    const double gamma = a.gamma != nullptr ? (double)a.gamma[c] : 1.0;
+    m1 = fma(gamma, s0, m1);
+    m2 = fma(gamma, s1, m2);
   }
   m1 = block_total(m1, shared);
   m2 = block_total(m2, shared);
-  const float n = (float)g.P * (float)g.cg;
-  if (threadIdx.x == 0) a.moments[blockIdx.x] = make_float2(m1 / n, m2 / n);
+  const double n = (double)g.P * g.cg;
+  if (threadIdx.x == 0) a.moments[blockIdx.x] = make_float2((float)(m1 / n), (float)(m2 / n));
 }
 // Sums the rows of channel sums in a fixed order: a workgroup takes 8 channels (one 64-byte piece of a row), 128 threads
-// share a channel's rows.  Latency-bound: 4 us for 512 to 1024 rows of 32 channels (256 KB), a launch included.
+// share a channel's rows, of which a thread may have thousands: eight at a time go into 64 bits.  Latency-bound: 4 us for 512
+// to 1024 rows of 32 channels (256 KB), a launch included.
 __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const NormArgs a) {
   __shared__ float2 shared[16][8];
   const int k = threadIdx.x & 7, r = threadIdx.x >> 3, c = blockIdx.x * 8 + k;
-  float2 s = make_float2(0.f, 0.f);
+  double s0 = 0.0, s1 = 0.0;
   if (c < a.g.C) {
     for (int row = r; row < a.chan_rows; row += 128 * 8) {       // eight loads in flight: the kernel is one memory latency long
       float2 p[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[i] = a.chan[(int64_t)min(row + i * 128, a.chan_rows - 1) * a.chan_stride + c];
+      float2 eight = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        s.x += row + i * 128 < a.chan_rows ? p[i].x : 0.f;
-        s.y += row + i * 128 < a.chan_rows ? p[i].y : 0.f;
+        eight.x += row + i * 128 < a.chan_rows ? p[i].x : 0.f;
+        eight.y += row + i * 128 < a.chan_rows ? p[i].y : 0.f;
       }
+      s0 += (double)eight.x;
+      s1 += (double)eight.y;
     }
   }
+  float2 s = make_float2((float)s0, (float)s1);
 #pragma unroll
   for (int o = 32; o >= 8; o >>= 1) {
     s.x += __shfl_xor(s.x, o, 64);
