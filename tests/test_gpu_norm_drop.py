@@ -876,3 +876,21 @@ def test_gradients_of_one_sign(ua, dtype, shape, bias):
     within(db, want.expand(C), K * U * want.expand(C), "dbias of a constant")
     del ones, dy
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("C, G", [(512, 8), (1040, 1)])          # one workgroup; the general kernels
+def test_gelu_in_fp32(ua, C, G):
+    """The function and its slope by themselves: gamma = 0 makes z = beta, one image of one pixel makes dbias the slope.
+    1 - Phi is fitted to 1.1e-8 or, below 1e-3, to 1.1e-5 of itself; t, the polynomial, their product and 2^x round 3 + 4 + 2 + 2
+    times, 2^x's argument (z^2 / 2 log2 e, twice rounded) z^2 u; then 1 - (1 - Phi), the Gaussian's factors and one rounding each."""
+    z = torch.linspace(-13, 8, C)
+    zero, one = torch.zeros(C).cuda(), torch.ones(1, 1, 1, C).cuda()
+    x = place(rnd(1, 1, 1, 1, C), torch.float32)
+    y, m, r = ua.ops.group_norm_act_fwd(x, C, G, zero, z.cuda(), act="gelu")
+    _, _, db = ua.ops.group_norm_act_bwd(x, place(one.cpu(), torch.float32), m, r, C, G, zero, z.cuda(), act="gelu")
+    z = z.double()
+    tail, phi, gauss = 0.5 * torch.erfc(z.abs() * 0.5 ** 0.5), 0.5 * torch.erfc(-z * 0.5 ** 0.5), torch.exp(-0.5 * z * z) / (2 * np.pi) ** 0.5
+    dphi = torch.minimum(torch.tensor(1.1e-8, dtype=torch.float64), 1.1e-5 * tail) + (11 + z * z) * U * tail + U * phi
+    within(y[0, 0, 0, :C], z * phi, z.abs() * dphi + U * (z * phi).abs() + 1e-37, "value")
+    slope = phi + z * gauss
+    within(db, slope, dphi + (z * gauss).abs() * (5 + z * z) * U + U * slope.abs() + 1e-37, "slope")

@@ -61,29 +61,42 @@ template <typename F> __device__ __forceinline__ F wave_total(F v) {
 // where it meets a factor that falls faster than |v| grows (z^2 s (1 - s) < 0.5, z^2 exp(-z^2 / 2) < 0.75).
 __device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 __device__ __forceinline__ float sigmoid_fast(float z) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-z)); }
-// Phi(z) and exp(-z^2 / 2).  erf by formula 7.1.26 of Abramowitz and Stegun, "Handbook of Mathematical Functions"
-// (error at most 1.5e-7, 2.5 half steps of fp32 at 1): its exponential is the Gaussian that the slope needs.  Its argument
-// |z| / sqrt 2 and the half of 1 - Phi(|z|) = (1 - erf) / 2 are in the constants.
-__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.231641888f, fabsf(z), 1.f)), e = __builtin_amdgcn_exp2f(z * -0.72134752f * z);
-  float p = fmaf(0.5307027145f, t, -0.7265760135f);
-  p = fmaf(p, t, 0.7107068705f);
-  p = fmaf(p, t, -0.142248368f);
-  p = fmaf(p, t, 0.127414796f);
+// Phi(z) and exp(-z^2 / 2), from (1 - Phi(|z|)) exp(z^2 / 2) / t as a polynomial in t = 1 / (1 + k |z|); its exponential is the
+// Gaussian that the slope needs.  Tensors of N values a vector:
+//   4, fp32: degree 6, fitted here for the least maximum of the error over max(1 - Phi, 10^-3), k = 0.34: 1 - Phi is off by at most
+//   1.1e-8, a fifth of fp32's half step at 1, or 1.1e-5 of itself where it is smaller than 10^-3;
+//   8, bf16: degree 4, erf by formula 7.1.26 of Abramowitz and Stegun, "Handbook of Mathematical Functions", k, 1 / sqrt 2 and the
+//   half of 1 - Phi = (1 - erf) / 2 in the constants: off by at most 7.5e-8, a 2^-15th of bf16's half step at 1.
+template <int N> __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(N == 4 ? 0.34f : 0.231641888f, fabsf(z), 1.f)), e = __builtin_amdgcn_exp2f(z * -0.72134752f * z);
+  float p;
+  if constexpr (N == 4) {
+    p = fmaf(0.0441167168f, t, -0.197348997f);
+    p = fmaf(p, t, 0.258327425f);
+    p = fmaf(p, t, -0.0253811497f);
+    p = fmaf(p, t, 0.153916016f);
+    p = fmaf(p, t, 0.130408421f);
+    p = fmaf(p, t, 0.135961592f);
+  } else {
+    p = fmaf(0.5307027145f, t, -0.7265760135f);
+    p = fmaf(p, t, 0.7107068705f);
+    p = fmaf(p, t, -0.142248368f);
+    p = fmaf(p, t, 0.127414796f);
+  }
   const float tail = p * t * e;                                  // 1 - Phi(|z|)
   *gauss = e;
   return z >= 0.f ? 1.f - tail : tail;
 }
-template <int ACT> __device__ __forceinline__ float act_value(float z) {
+template <int ACT, int N> __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == MI_ACT_RELU) return __builtin_elementwise_maximum(z, 0.f);   // a NaN stays one
   if constexpr (ACT == MI_ACT_SILU) return z * sigmoid_fast(z);
   if constexpr (ACT == MI_ACT_GELU) {
     float e;
-    return z * normal_cdf(z, &e);
+    return z * normal_cdf<N>(z, &e);
   }
   return z;
 }
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
+template <int ACT, int N> __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == MI_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == MI_ACT_SILU) {
     const float s = sigmoid_fast(z);
@@ -91,7 +104,7 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z) {
   }
   if constexpr (ACT == MI_ACT_GELU) {
     float e;
-    const float phi = normal_cdf(z, &e);
+    const float phi = normal_cdf<N>(z, &e);
     return fmaf(z * 0.39894228f, e, phi);
   }
   return 1.f;
@@ -297,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const NormArgs a) {
     if (a.drop.on && !a.drop.per_channel) keep.add(0, a.drop, offset, ((uint64_t)w.b * g.P + p) * (uint32_t)(g.nv * N) + c0);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      f[j] = act_value<ACT>(fmaf((f[j] - mean[j]) * rstd[j], gamma[j], beta[j]));
+      f[j] = act_value<ACT, N>(fmaf((f[j] - mean[j]) * rstd[j], gamma[j], beta[j]));
       if (a.drop.on) f[j] = keep.kept(0, j, f[j] * a.drop.scale);
       if (c0 + j >= g.C) f[j] = 0.f;
     }
@@ -726,7 +739,7 @@ __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I >
       float f[N];
       ActVec<T>::unpack(v[i], f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = act_value<decltype(act)::value>(fmaf(f[j] - mean[j / Q], gamma[j], beta[j]));
+      for (int j = 0; j < N; ++j) f[j] = act_value<decltype(act)::value, N>(fmaf(f[j] - mean[j / Q], gamma[j], beta[j]));
       if (a.drop.on) {
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = keep.kept(i, j, f[j] * a.drop.scale);
@@ -757,7 +770,7 @@ __device__ __forceinline__ void norm_dz(const NormArgs& a, const float* x, const
       z = (float)(((double)x[j] - (double)mean[j]) * (double)rstd[j] * (double)gamma[j] + (double)beta[j]);
     float d = dy[j];
     if (a.drop.on) d = keep.kept(0, j, d * a.drop.scale);
-    dz[j] = ACT == MI_ACT_RELU ? (z > 0.f ? d : 0.f) : d * act_slope<ACT>(z);
+    dz[j] = ACT == MI_ACT_RELU ? (z > 0.f ? d : 0.f) : d * act_slope<ACT, N>(z);
   }
 }
 template <typename T>
@@ -1001,7 +1014,7 @@ __device__ __forceinline__ void bwd_step(u32x4_t x4, u32x4_t& d4, u32x4_t& low, 
     for (int j = 0; j < 4; ++j) x[j] = fmaf(x[j], unit[(4 * e + j) * NS / N], -mean[(4 * e + j) * NS / N]);
     if constexpr (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[4 * e + j], beta[4 * e + j]));
+      for (int j = 0; j < 4; ++j) d[j] *= act_slope<ACT, N>(fmaf(x[j], scaled[4 * e + j], beta[4 * e + j]));
     }
     if constexpr (N == 4 && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) ActVec<T>::pack4(d, e, d4);
     if constexpr (SPLIT) {
@@ -1176,7 +1189,7 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
       for (int j = 0; j < 4; ++j) {
         const int c = 4 * e + j, k = c / Q;
         x[j] = fmaf(x[j], unit[k], -mean[k]);
-        if constexpr (N == 8 && !SPLIT && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT>(fmaf(x[j], scaled[c], beta[c]));
+        if constexpr (N == 8 && !SPLIT && (ACT == MI_ACT_SILU || ACT == MI_ACT_GELU)) d[j] *= act_slope<ACT, N>(fmaf(x[j], scaled[c], beta[c]));
         d[j] = fmaf(x[j], b1[k], fmaf(d[j], slope[c], b0[k]));
       }
       if (ragged) {
