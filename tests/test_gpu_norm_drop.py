@@ -894,3 +894,55 @@ def test_gelu_in_fp32(ua, C, G):
     within(y[0, 0, 0, :C], z * phi, z.abs() * dphi + U * (z * phi).abs() + 1e-37, "value")
     slope = phi + z * gauss
     within(db, slope, dphi + (z * gauss).abs() * (5 + z * z) * U + U * slope.abs() + 1e-37, "slope")
+
+
+@pytest.mark.parametrize("shape", [(2, 33, 31, 32, 8), (3, 1, 2, 64, 8), (9, 100, 96, 40, 8), (1, 256, 255, 66, 3)])
+def test_norm_far_from_zero_forward_and_backward(ua, shape):
+    """A mean 10^4 standard deviations from zero: y is off by the mean's one rounding, U |mean| rstd, besides what it is anywhere
+    (with deviations of size 1 in place of |x| in the additions: those are sums of deviations); dx, from the statistics handed on,
+    by nothing else."""
+    B, H, W, C, G = shape
+    ops = ua.ops
+    x, dy = rnd(1, B, H, W, C) + 1e4, rnd(5, B, H, W, C, scale=0.1)
+    gamma, beta = rnd(3, C, scale=0.3, shift=1.0), rnd(4, C, scale=0.3)
+    y, mean, rstd = ops.group_norm_act_fwd(place(x, torch.float32), C, G, gamma.cuda(), beta.cuda())
+    x6, g6, b6 = x.double(), gamma.double(), beta.double()
+    oy, om, orr, z = N.group_norm_act_fwd(x6, G, g6, b6, "none", float(torch.tensor(1e-5)))
+    cg = C // G
+    deviations = x6 - N._per_channel(om, cg)
+    bound = fwd_bound(deviations, oy, z, torch.zeros_like(om), orr, g6, b6, G, torch.float32)
+    within(y[..., :C], oy, bound + N._per_channel(U * om.abs() * orr, cg) * g6.abs(), "y")
+    out = ops.group_norm_act_bwd(place(x, torch.float32), place(dy, torch.float32), mean, rstd, C, G, gamma.cuda(), beta.cuda(), act="silu")
+    bwd_check(out, x6, dy.double(), mean.double().cpu(), rstd.double().cpu(), G, g6, b6, "silu", None, torch.float32, "backward")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("polls", [-1, 0])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_non_finite_values_where_workgroups_share(ua, monkeypatch, dtype, polls, bad):
+    """A value that is no number, in x or in dy, stays in its group and image: images of several parts, the general kernels."""
+    ops = ua.ops
+    monkeypatch.setattr(ops, "_POLLS", polls)
+    for B, H, W, C, G in ((9, 100, 96, 40, 5), (12, 90, 80, 64, 4), (1, 256, 255, 72, 3)):
+        x, dy = rnd(1, B, H, W, C).to(dtype), rnd(2, B, H, W, C).to(dtype)
+        w, b = rnd(3, C, scale=0.3, shift=1.0).cuda(), rnd(4, C).cuda()
+        cg, c = C // G, C // G + 1                                # group 1
+        hit = torch.zeros(B, H, W, N.pad_ch(C), dtype=torch.bool)
+        hit[-1, ..., cg:2 * cg] = True
+        for act in ("relu", "silu"):
+            def run(x, dy):
+                y, m, r = ops.group_norm_act_fwd(place(x, dtype), C, G, w, b, act=act)
+                return (y, m, r) + ops.group_norm_act_bwd(place(x, dtype), place(dy, dtype), m, r, C, G, w, b, act=act)
+            clean = run(x, dy)
+            bad_x, bad_dy = x.clone(), dy.clone()
+            bad_x[-1, H - 1, W - 2, c] = bad
+            bad_dy[-1, H // 2, 3, c] = bad
+            y, m, r, dx, dw, db = run(bad_x, dy)
+            assert torch.equal(y.cpu()[~hit], clean[0].cpu()[~hit]) and torch.isnan(y.cpu()[hit]).all()
+            assert torch.equal(dx.cpu()[~hit], clean[3].cpu()[~hit])
+            assert not torch.isfinite(m[-1, 1]) and not torch.isfinite(r[-1, 1]) and int(torch.isfinite(r).sum()) == B * G - 1
+            dx, dw, db = run(x, bad_dy)[3:]
+            assert torch.equal(dx.cpu()[~hit], clean[3].cpu()[~hit])
+            for got, want in ((dw, clean[4]), (db, clean[5])):
+                others = torch.arange(C) != c
+                assert torch.equal(got.cpu()[others], want.cpu()[others])

@@ -21,7 +21,8 @@
 // Precision of the statistics: the corrected two-pass form (Chan, Golub, LeVeque, "Algorithms for computing the sample
 // variance", 1983).  A tile's mean m comes first, from registers; then r = sum (x - m) and q = sum (x - m)^2, which give
 // the mean m + r / n and the squared deviations q - r^2 / n without m's own rounding; tiles are joined in 64 bits.  Data
-// far from zero lose nothing: at a mean of 10^4 standard deviations rstd is off by 1e-7, without r by 2e-5.
+// far from zero cost the statistics nothing: at a mean of 10^4 standard deviations rstd is off by 1e-7, without r by 2e-5.  The
+// mean is handed on in fp32, as the backward pass gets it: its rounding, 2^-24 |mean| rstd, is in h and y.
 // Sums have a fixed order: results repeat bit for bit.
 #pragma once
 #include "drop.h"
