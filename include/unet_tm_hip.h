@@ -197,8 +197,9 @@ int mi_dropout_fwd(const void* x, int x_cstride, int x_coff, const void* residua
 #define MI_ACT_GELU 3
 /* y = dropout(act((x - mean) * rstd * gamma + beta)): torch's nn.GroupNorm(groups, C, eps), an activation and a
  * dropout (drop may be NULL) in one operator.  gamma, beta: C floats each, or NULL (1 and 0).  mean, rstd
- * (B*groups floats each) are written; the backward pass reads them.  C must be a multiple of groups.  y must not
- * overlap x.  ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content (NULL where that is 0).
+ * (B*groups floats each) are written; the backward pass reads them.  Values up to 2^126 in magnitude are taken, also where
+ * their squares pass fp32's range.  C must be a multiple of groups.  y must not overlap x.
+ * ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content (NULL where that is 0).
  * Several workgroups may share a large image; each then looks for the others' sums, at most `polls` times, and forms
  * those that have not come itself, so that no call depends on its workgroups running at the same time.  polls < 0: the
  * library's choice (some milliseconds).  The result does not depend on it, bit for bit. */
@@ -214,6 +215,7 @@ int mi_group_norm_act_bwd(const void* x, int x_cstride, int x_coff, const void* 
                           void* dx, int dx_cstride, int dx_coff, float* dgamma, float* dbeta, float alpha, float beta_acc,
                           int B, int H, int W, int C, int groups, int act, const mi_dropout* drop, int polls,
                           void* ws, size_t ws_bytes, int dtype, mi_stream s);
+/* 0 also for shapes and types that the calls above refuse. */
 size_t mi_group_norm_ws_bytes(int B, int H, int W, int C, int groups, int backward, int dtype);
 
 /* ------------------------------------------------------------------ A6: MSE loss */

@@ -121,8 +121,9 @@ inline int pow2_ceil(int64_t v) {
   return p;
 }
 // How the slab kernels divide the work, or false where they do not apply.
-// Up to 64 parts, which run at the same time on a fraction of the card.  Without parts, by the general kernels: 16 images of 128x128x64
-// bf16 20 us forward and 75 backward, with them 14 and 25; 2 of 256x256x32 12.7 and 50 against 13.6 and 20.
+// Up to 64 parts, which run at the same time on a fraction of the card; more have not been measured since the parts of an image
+// start next to each other.  Without parts, by the general kernels: 16 images of 128x128x64 bf16 25 us forward and 48 backward,
+// with them 17 and 28; 2 of 256x256x32 14 and 24 against 12 and 17; 1024 of 64x64x32 154 and 286 against 109 and 176.
 constexpr int kMaxParts = 64;
 constexpr int kPolls = 4096;                 // about 1 us each
 // The division with `iters` vectors a thread of chunks of cv vectors, up to `most` threads for an image, `most_nb` for several.
@@ -165,8 +166,9 @@ inline bool choose_slab(const NormGeom& g, int N, bool backward, Slab* out) {
   // chunk then has a workgroup of its own.  Measured, forward / backward: 8 images of 4x4x1024 fp32 4.0 / 7.0 us with whole
   // pixels, 3.7 / 6.5 so; 32 of 16x16x64 bf16 6.0 / 11.3 with 128 bytes, 4.3 / 8.1 with 64 (with 32: 5.0 / 8.7); but
   // 16 of 128x128x64 bf16, which have parts, 14.1 / 24.3 with 128 bytes and 18.8 / 38 with 64.
-  // Backward, an image of more than 64 parts is cut into narrower chunks whatever their number: one of 256x256x512 fp32 616 us
-  // by the general kernels, 151 in chunks of 64 bytes, 16 of 256x256x64 bf16 225 and 124; forward 120 and 146, 88 and 106.
+  // Backward, an image of more than 64 parts is cut into narrower chunks whatever their number: one of 256x256x512 fp32 223 us
+  // by the general kernels, 145 in chunks of 64 bytes, 16 of 256x256x64 bf16 133 and 110, 256 of 70x70x256 fp32 1168 and 607.
+  // Forward the same gives 86 and 103, 76 and 81, but 739 and 467: not taken, though large batches of wide pixels would gain.
   for (;;) {
     const int64_t lanes = pow2_ceil(cv), size = g.P * lanes, wgs = (int64_t)g.B * ((g.nv + cv - 1) / cv);
     int64_t half = cv / 2 / unit * unit;

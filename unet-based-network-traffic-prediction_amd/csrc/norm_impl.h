@@ -561,8 +561,8 @@ __device__ __forceinline__ uint64_t get_word(const uint64_t* p) {
 // parts in an order that depends on their number alone, and `take(group, s0, s1, part 0's first word)` gets these.  Returns the
 // number of a part that has not come, or -1.
 // Threads are (share of the parts, group), up to 64 groups at a time, so that the words of several parts are under way together
-// and few sums cross lanes (with the parts along a wave's lanes and one group after the other, 64 images of 100x100x64 fp32 in
-// 64 groups took 116 us forward and 127 backward, so 91 and 106).
+// and few sums cross lanes (64 images of 100x100x64 fp32 in 64 groups, before and after this change alone: with the parts along a
+// wave's lanes and one group after the other 116 us forward and 127 backward, so 91 and 106).
 template <int W, typename Term, typename Take>
 __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeom& g, const Slab& s, int groups, int* missing,
                                             double2* partial, Term term, Take take) {
@@ -633,10 +633,11 @@ __device__ __forceinline__ int slab_collect(const uint64_t* words, const NormGeo
 // other threads -- is several hundred instructions, worth it for 128 values (512 threads with 8 vectors, forward: 16.3 us
 // against 16.4 for 512 images of 32x32x32 bf16).  16 vectors leave three workgroups a CU (up to 168 registers); 4 vectors
 // stay within 128, so 1024 threads fit.
-// Bound by HBM: 1024 images of 64x64x32 bf16 with SiLU, four parts each, 103 us for 537 MB = 5.2 TB/s, and 2 us for the launch
-// that empties the words; 512 of 32x32x32 with ReLU and dropout 10 % 14.3 us for 67 MB = 4.7 TB/s (the mask's words are
-// worked out while the loads are in flight).  One image of 64x64x32: 8 us, of which a launch is 2.8 and the rest one
-// memory latency after the other.
+// Bound by HBM.  Medians of a kernel trace over rotating tensors: 1024 images of 64x64x32 bf16 with SiLU, four parts each, 108 us
+// for 537 MB = 5.0 TB/s, and 4.8 for the launch that empties the words (105 a call for both, back to back); 512 of 32x32x32 with
+// ReLU and dropout 10 % 16.4 us for 67 MB = 4.1 TB/s (14.9 a call: the mask's words are worked out while the loads are in
+// flight); 512 of 64x64x32 fp32 with SiLU 101 for 537 MB = 5.3 TB/s.  One image of 64x64x32: 8.5 us, of which a launch is 2.8
+// and the rest one memory latency after the other.
 template <typename T, int NS, int I, bool PARTS>
 __global__ __launch_bounds__(I == 4 && !PARTS ? kWideThreads : kSlabThreads, I > 4 || PARTS ? 3 : 4) void gn_fwd_slab_kernel(const NormArgs a, const Slab s) {
   constexpr int N = ActVec<T>::N, Q = N / NS;
@@ -1207,11 +1208,12 @@ __device__ __forceinline__ void bwd_emit(const NormArgs& a, const Slab& s, const
 // group's two sums are made of them.  Dropout's factor is left out of dz and t until the end: dx and the gradients are
 // linear in it.
 // 16 vectors of x and of dy take 128 registers, all of it up to 256: two workgroups a CU.  Those load together, compute
-// together and store together, so the time is near the sum of both: 64 images of 128x128x32 bf16 with SiLU 45 us for 201 MB
-// (32 of memory at 6.2 TB/s), 512 of 32x32x32 with ReLU and dropout 20 for 101 MB (16).
+// together and store together, so the time is near the sum of both.  Medians of a kernel trace over rotating tensors: 64 images of
+// 128x128x32 bf16 with SiLU 47 us for 201 MB (32 of memory at 6.2 TB/s), 512 of 32x32x32 with ReLU and dropout 24 for 101 MB (16),
+// 256 of 64x64x32 fp32 with ReLU 76 for 403 MB (65).
 // SPLIT: the second pass takes dz as the first one had it, in fp32: its upper halves are where dy was, its lower ones in LDS
-// (64 KB; each thread its own, nothing to wait for).  Working the slope out again instead took 51 us, and for 1024 images of
-// 64x64x32 with GELU 255 where it is 185 now; the bits are the same.  Where a bf16 vector has eight pieces there is no LDS to
+// (64 KB; each thread its own, nothing to wait for).  Working the slope out again instead took 60 us where it was 53.5 with this
+// change alone, and for 1024 images of 64x64x32 with GELU 255 and 185; the bits are the same.  Where a bf16 vector has eight pieces there is no LDS to
 // spare beside the sums of two workgroups, and with 4 vectors a thread nothing to gain.
 // What did not help there: 8 vectors a thread and three workgroups, a staggered start, workgroups that stay and prefetch
 // the next part (their polls and stores queue behind the prefetch: 83 us against 62), loads of x and dy in turn.
