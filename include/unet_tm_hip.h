@@ -198,7 +198,8 @@ int mi_dropout_fwd(const void* x, int x_cstride, int x_coff, const void* residua
 /* y = dropout(act((x - mean) * rstd * gamma + beta)): torch's nn.GroupNorm(groups, C, eps), an activation and a
  * dropout (drop may be NULL) in one operator.  gamma, beta: C floats each, or NULL (1 and 0).  mean, rstd
  * (B*groups floats each) are written; the backward pass reads them.  Values up to 2^126 in magnitude are taken, also where
- * their squares pass fp32's range.  C must be a multiple of groups.  y must not overlap x.
+ * their squares pass fp32's range; with eps = 0 a group's deviations must be above 2^-50, whose squares it still holds.
+ * C must be a multiple of groups.  y must not overlap x.
  * ws: mi_group_norm_ws_bytes(..., 0, ...) bytes, any content (NULL where that is 0).
  * Several workgroups may share a large image; each then looks for the others' sums, at most `polls` times, and forms
  * those that have not come itself, so that no call depends on its workgroups running at the same time.  polls < 0: the

@@ -946,3 +946,13 @@ def test_non_finite_values_where_workgroups_share(ua, monkeypatch, dtype, polls,
             for got, want in ((dw, clean[4]), (db, clean[5])):
                 others = torch.arange(C) != c
                 assert torch.equal(got.cpu()[others], want.cpu()[others])
+
+
+def test_dropout_goes_backward_twice(ua):
+    """Its node keeps no tensor unless it has a counter, so it needs no retain_graph."""
+    x, drop = rnd(1, 2, 4, 4, 64).cuda().requires_grad_(), ua.ops.Drop(0.5, 1)
+    y = ua.dropout(x, 64, drop)
+    dy = rnd(2, 2, 4, 4, 64).cuda()
+    first, = torch.autograd.grad(y, x, dy)
+    again, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(first, again) and torch.equal(first, ua.ops.dropout_bwd(dy, 64, drop))

@@ -50,7 +50,8 @@ class _GroupNormActFunction(torch.autograd.Function):
 class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, channels, drop):
-        ctx.save_for_backward(_counter(drop))
+        if _counter(drop) is not None:             # nothing else is saved: without one, backward may run as often as it likes
+            ctx.save_for_backward(drop.offset_dev)
         ctx.spec, ctx.width = (channels, drop), x.shape[3]
         ctx.residual_width = residual.shape[3] if residual is not None else 0
         return ops.dropout_fwd(x, channels, drop, residual=residual)
@@ -58,8 +59,9 @@ class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _ = ctx.saved_tensors                      # raises where the counter was changed
         channels, drop = ctx.spec
+        if _counter(drop) is not None:
+            _ = ctx.saved_tensors                  # raises where the counter was changed
         dy = dy.contiguous()
         dx = _widened(ops.dropout_bwd(dy, channels, drop), ctx.width) if ctx.needs_input_grad[0] else None
         dr = None
